@@ -434,6 +434,47 @@ int pydtnn_hip_bn_training_bwd_f64(const double *dy, const double *xn, const dou
                                    void *stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Operators for several element types.  `dtype` names the type of the tensors; vectors per channel and
+ * statistics are float32, or float64 where the tensors are.  None of them has a counterpart in PyDTNN.
+ * ---------------------------------------------------------------------------------------- */
+#define PYDTNN_HIP_DTYPE_F32 0
+#define PYDTNN_HIP_DTYPE_F64 1
+#define PYDTNN_HIP_DTYPE_F16 2
+#define PYDTNN_HIP_DTYPE_BF16 3
+
+/* Group normalisation with an activation.  x is (images, pixels, channels) where nhwc != 0, else
+ * (images, channels, pixels); a group is channels / groups consecutive channels over all pixels of an image.
+ *   forward : mean, inv_std = 1 / sqrt(var + eps) of each group (images, groups), var without Bessel's correction;
+ *             z = gamma[c] * (x - mean) * inv_std + beta[c];  y = z, z > 0 ? z : 0 or z / (1 + exp(-z)).
+ *   backward: from dy, x and the forward's mean and inv_std: dgamma, dbeta (channels) and, unless it is NULL, dx.
+ *             Where the activation is PYDTNN_HIP_ACT_RELU, dy counts where z, computed from these inputs, is positive.
+ * Sums are taken in a fixed order.  Outputs may not overlap inputs.  channels has to be a multiple of groups; pixels and
+ * channels are at most 2^30 (PYDTNN_HIP_ERR_UNSUPPORTED).  Workspace: pydtnn_hip_gn_workspace_bytes(...) with the same
+ * extents; backward = 0 or 1. */
+#define PYDTNN_HIP_ACT_IDENTITY 0
+#define PYDTNN_HIP_ACT_RELU 1
+#define PYDTNN_HIP_ACT_SILU 2
+size_t pydtnn_hip_gn_workspace_bytes(int dtype, int nhwc, int backward, long images, long channels, long pixels,
+                                     long groups);
+int pydtnn_hip_gn_forward(int dtype, int nhwc, const void *x, const void *gamma, const void *beta, void *y, void *mean,
+                          void *inv_std, long images, long channels, long pixels, long groups, double eps,
+                          int activation, void *workspace, size_t workspace_bytes, void *stream);
+int pydtnn_hip_gn_backward(int dtype, int nhwc, const void *dy, const void *x, const void *gamma, const void *beta,
+                           const void *mean, const void *inv_std, void *dgamma, void *dbeta, void *dx, long images,
+                           long channels, long pixels, long groups, int activation, void *workspace,
+                           size_t workspace_bytes, void *stream);
+
+/* Dropout whose mask is a function of (seed, offset, index of the element); it is never stored, and the backward pass
+ * is the same call on dy.  Philox4x32-10 with key = seed and counter = (index / 8, offset) (low words first) gives the
+ * 16-bit numbers of eight consecutive elements, low halves first.  With threshold = rate * 2^16 rounded to a whole number
+ * (to even between two), an element is kept when its number is >= threshold and then multiplied by
+ * 2^16 / (2^16 - threshold), the reciprocal of the probability that it is kept; it is 0 otherwise, whatever x holds.
+ * `offset_dev`, unless it is NULL, is a number on the device that is added to `offset`: a captured graph whose number
+ * changes between replays draws another mask each time.  y may be x.  0 <= rate <= 1. */
+int pydtnn_hip_dropout(int dtype, const void *x, void *y, long total, double rate, uint64_t seed, uint64_t offset,
+                       const int64_t *offset_dev, void *stream);
+
+/* ------------------------------------------------------------------------------------------
  * Host-pointer compatibility flavour (exported by libconvGemm.so only).  Signatures are those
  * PyDTNN's ctypes shim calls (pydtnn/backends/cpu/libs/conv_gemm.py:91-92, :191-205, :234-248,
  * :299-307, :321-328).  ac_pack / bc_pack are accepted and ignored; alloc_pack_buffs hands out two

@@ -660,18 +660,36 @@ class Flatten(Layer):
 
 
 class Dropout(Layer):
-    """pydtnn/backends/cpu/layers/dropout_cpu.py:28-43 (mask drawn with torch's generator on the GPU)."""
+    """pydtnn/backends/cpu/layers/dropout_cpu.py:28-43 (mask drawn with torch's generator on the GPU).
 
-    def __init__(self, rate=0.5):
+    With a ``seed`` (0 <= seed < 2^32) the mask is a function of the seed, the layer's id and the number of its training
+    steps so far, and is stored nowhere: the backward pass draws it again.  ``step`` holds that number on the GPU, counted up
+    by each forward pass in TRAIN_MODE (also by each replay of a captured one); setting it resumes a run where it was."""
+
+    def __init__(self, rate=0.5, seed=None):
         super().__init__()
         self.rate = min(1., max(0., rate))
+        if seed is not None and not 0 <= seed < 1 << 32:
+            raise ValueError("the seed of a Dropout layer is a number of 32 bits")
+        self.seed = seed
         self.mask = None
+        self.step = None
+        self._dropped = False
 
     def initialize(self, prev_shape, need_dx=True):
         super().initialize(prev_shape, need_dx)
         self.shape = prev_shape
+        if self.seed is not None:
+            self.step = torch.zeros(1, dtype=torch.int64, device="cuda")
+
+    def _key(self):
+        return self.seed + (self.id << 32)
 
     def forward(self, x):
+        self._dropped = self.seed is not None and self.model.mode == TRAIN_MODE and self.rate > 0
+        if self._dropped:
+            self.step += 1
+            return ops.dropout(x, self.rate, self._key(), self.step)
         if self.model.mode == TRAIN_MODE and self.rate > 0:
             self.mask = torch.bernoulli(torch.full_like(x, 1 - self.rate)) / (1 - self.rate)
             return x * self.mask
@@ -680,7 +698,52 @@ class Dropout(Layer):
 
     def backward(self, dy):
         if self.need_dx:
+            if self._dropped:
+                return ops.dropout_backward(dy, self.rate, self._key(), self.step)
             return dy if self.mask is None else dy * self.mask
+
+
+# --------------------------------------------------------------------------- GroupNormalization
+class GroupNormalization(Layer):
+    """Normalises each image's groups of consecutive channels over their pixels, scales and shifts each channel and applies
+    ``activation`` ("", "relu" or "silu") in the same kernels, in either tensor format and in either mode.  The backward pass
+    keeps the layer's input and two numbers a group, nothing of the size of the output."""
+
+    def __init__(self, groups=32, beta=0.0, gamma=1.0, epsilon=1e-5, activation=""):
+        super().__init__()
+        self.groups = groups
+        self.beta_init_val = beta
+        self.gamma_init_val = gamma
+        self.epsilon = epsilon
+        self.activation = activation
+        self.grad_vars = {"beta": "dbeta", "gamma": "dgamma"}
+        self.gamma = self.beta = self.dgamma = self.dbeta = None
+        self.x = self.mean = self.inv_std = None
+
+    def initialize(self, prev_shape, need_dx=True):
+        super().initialize(prev_shape, need_dx)
+        self.shape = prev_shape
+        channels = decode_tensor(prev_shape, self.model.tensor_format)[-1]
+        if self.groups < 1 or channels % self.groups:
+            raise ValueError(f"{channels} channels do not make {self.groups} groups")
+        self.gamma = torch.full((channels,), self.gamma_init_val, dtype=self.model.dtype, device="cuda")
+        self.beta = torch.full((channels,), self.beta_init_val, dtype=self.model.dtype, device="cuda")
+        self.nparams = 2 * channels
+
+    def _nhwc(self):
+        return len(self.shape) < 3 or self.model.tensor_format != PYDTNN_TENSOR_FORMAT_NCHW
+
+    def forward(self, x):
+        y, mean, inv_std = ops.gn_forward(x, self.gamma, self.beta, self.groups, self.epsilon, self.activation,
+                                          self._nhwc())
+        if self.model.mode == TRAIN_MODE:
+            self.x, self.mean, self.inv_std = x, mean, inv_std
+        return y
+
+    def backward(self, dy):
+        self.dgamma, self.dbeta, dx = ops.gn_backward(dy, self.x, self.gamma, self.beta, self.mean, self.inv_std,
+                                                      self.groups, self.activation, self._nhwc(), need_dx=self.need_dx)
+        return dx
 
 
 # --------------------------------------------------------------------------- BatchNormalization (inference)

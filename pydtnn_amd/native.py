@@ -18,6 +18,9 @@ OP_FWD, OP_DW, OP_DX, OP_DX_I2C, OP_DB, OP_FWD_I2C = range(6)
 # status codes of include/pydtnn_hip.h
 PYDTNN_HIP_OK, PYDTNN_HIP_ERR_INVALID, PYDTNN_HIP_ERR_WORKSPACE, PYDTNN_HIP_ERR_LAUNCH, PYDTNN_HIP_ERR_UNSUPPORTED = range(5)
 
+# values of its `dtype` arguments
+DTYPES = {torch.float32: 0, torch.float64: 1, torch.float16: 2, torch.bfloat16: 3}
+
 _c = ctypes
 _f32p, _i8p, _i32p, _vp = _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p
 _geom13_i = [_c.c_int] * 13
@@ -108,6 +111,13 @@ SIGNATURES = {
     "pydtnn_hip_bn_training_fwd_f64": (_c.c_int, [_vp] * 8 + [_c.c_double, _c.c_double, _c.c_long, _c.c_int, _c.c_long,
                                                             _vp]),
     "pydtnn_hip_bn_training_bwd_f64": (_c.c_int, [_vp] * 7 + [_c.c_long, _c.c_int, _c.c_long, _vp]),
+    # several element types
+    "pydtnn_hip_gn_workspace_bytes": (_c.c_size_t, [_c.c_int] * 3 + [_c.c_long] * 4),
+    "pydtnn_hip_gn_forward": (_c.c_int, [_c.c_int, _c.c_int] + [_vp] * 6 + [_c.c_long] * 4 + [_c.c_double, _c.c_int, _vp,
+                                                                                         _c.c_size_t, _vp]),
+    "pydtnn_hip_gn_backward": (_c.c_int, [_c.c_int, _c.c_int] + [_vp] * 9 + [_c.c_long] * 4 + [_c.c_int, _vp, _c.c_size_t,
+                                                                                          _vp]),
+    "pydtnn_hip_dropout": (_c.c_int, [_c.c_int, _vp, _vp, _c.c_long, _c.c_double, _c.c_uint64, _c.c_uint64, _vp, _vp]),
 }
 
 # Host-pointer flavour exported by libconvGemm.so with the reference's own names

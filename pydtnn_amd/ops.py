@@ -4,6 +4,9 @@ Names and argument order follow the reference's Cython modules and ``utils.matmu
 layer code (``layers.py``) reads like PyDTNN's CPU backend.  Every function enqueues work on the
 current HIP stream and returns freshly allocated device tensors.
 """
+import functools
+import math
+
 import torch
 
 from . import native
@@ -509,3 +512,138 @@ def conv_i2c_dx(nhwc, geom13, weights, dy, dx):
     check(lib().pydtnn_hip_conv_i2c_dx(int(nhwc), *geom13, f32(weights), f32(dy), f32(dx), ws, ws_bytes,
                                        stream_ptr()), "conv_i2c_dx")
     return dx
+
+
+# --------------------------------------------------------------------------- operators for several element types
+
+def _on_its_device(f):
+    """Runs ``f`` with the device of its first argument as the current one, so that the work goes to that device's
+    current stream."""
+    @functools.wraps(f)
+    def g(x, *args, **kwargs):
+        if x.is_cuda and x.device.index != torch.cuda.current_device():
+            with torch.cuda.device(x.device):
+                return f(x, *args, **kwargs)
+        return f(x, *args, **kwargs)
+    return g
+
+
+def _dtype_of(x):
+    code = native.DTYPES.get(x.dtype)
+    if code is None:
+        raise TypeError(f"Type '{x.dtype}' is not supported by this kernel (float32, float64, float16 or bfloat16)")
+    return code
+
+
+def _wide(dtype):
+    """The type of statistics and per-channel vectors of a tensor of type ``dtype``."""
+    return torch.float64 if dtype == torch.float64 else torch.float32
+
+
+def _need_like(x, dtype, **tensors):
+    """Each (tensor, shape) is of type ``dtype``, of that shape and on the device of ``x``."""
+    for name, (t, shape) in tensors.items():
+        if t.dtype != dtype:
+            raise TypeError(f"{name} is {t.dtype}, {dtype} expected")
+        if tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+        if t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, the other tensors on {x.device}")
+
+
+def _scratch(nbytes, x):
+    """Scratch memory of one call.  It is the caller's alone: under capture it belongs to the graph that is captured, and
+    no other graph or later call is handed the same memory while this one can still run."""
+    return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=x.device)
+
+
+_GN_ACTIVATIONS = {"": 0, None: 0, "relu": 1, "silu": 2}
+
+
+def _gn_extents(x, gamma, beta, groups, activation, nhwc):
+    """(images, channels, pixels, groups, activation) of a group normalisation of ``x``, checked."""
+    if activation not in _GN_ACTIVATIONS:
+        raise ValueError(f"group normalisation knows the activations 'relu' and 'silu', not {activation!r}")
+    if x.dim() < 2:
+        raise ValueError("group normalisation expects (batch, ..., channels) or (batch, channels, ...)")
+    channels = x.shape[-1] if nhwc else x.shape[1]
+    if groups < 1 or channels < 1 or channels % groups:
+        raise ValueError(f"{channels} channels do not make {groups} groups")
+    _need_like(x, _wide(x.dtype), gamma=(gamma, (channels,)), beta=(beta, (channels,)))
+    pixels = math.prod(x.shape[1:]) // channels
+    if pixels < 1:
+        raise ValueError(f"group normalisation of no pixels: x has shape {tuple(x.shape)}")
+    return x.shape[0], channels, pixels, groups, _GN_ACTIVATIONS[activation]
+
+
+@_on_its_device
+def gn_forward(x, gamma, beta, groups, eps=1e-5, activation="", nhwc=True):
+    """Group normalisation with an activation (None, "relu" or "silu"): y = act(gamma * (x - mean) * inv_std + beta) with
+    the statistics of each image's groups of consecutive channels, of shape (batch, groups).  ``x`` is (batch, ...,
+    channels), with ``nhwc=False`` (batch, channels, ...), in float32, float64, float16 or bfloat16; gamma, beta, mean and
+    inv_std are float32 (float64 for float64).  Returns (y, mean, inv_std)."""
+    dtype = _dtype_of(x)
+    images, channels, pixels, groups, act = _gn_extents(x, gamma, beta, groups, activation, nhwc)
+    if not eps >= 0:
+        raise ValueError(f"epsilon is {eps}, it has to be at least 0")
+    x = x.contiguous()
+    y = torch.empty_like(x)
+    mean = torch.empty((images, groups), dtype=gamma.dtype, device=x.device)
+    inv_std = torch.empty_like(mean)
+    if images:
+        nbytes = lib().pydtnn_hip_gn_workspace_bytes(dtype, int(nhwc), 0, images, channels, pixels, groups)
+        ws = _scratch(nbytes, x)
+        check(lib().pydtnn_hip_gn_forward(dtype, int(nhwc), ptr(x), ptr(gamma), ptr(beta), ptr(y), ptr(mean), ptr(inv_std),
+                                          images, channels, pixels, groups, float(eps), act, ptr(ws), nbytes, stream_ptr()),
+              "gn_forward")
+    return y, mean, inv_std
+
+
+@_on_its_device
+def gn_backward(dy, x, gamma, beta, mean, inv_std, groups, activation="", nhwc=True, need_dx=True):
+    """The gradients of ``gn_forward`` from its input and its two statistics -> (dgamma, dbeta, dx or None)."""
+    dtype = _dtype_of(x)
+    images, channels, pixels, groups, act = _gn_extents(x, gamma, beta, groups, activation, nhwc)
+    _need_like(x, x.dtype, dy=(dy, x.shape))
+    _need_like(x, gamma.dtype, mean=(mean, (images, groups)), inv_std=(inv_std, (images, groups)))
+    dy, x = dy.contiguous(), x.contiguous()
+    dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(gamma)
+    dx = torch.empty_like(x) if need_dx else None
+    if not images:
+        return dgamma.zero_(), dbeta.zero_(), dx
+    nbytes = lib().pydtnn_hip_gn_workspace_bytes(dtype, int(nhwc), 1, images, channels, pixels, groups)
+    ws = _scratch(nbytes, x)
+    check(lib().pydtnn_hip_gn_backward(dtype, int(nhwc), ptr(dy), ptr(x), ptr(gamma), ptr(beta), ptr(mean), ptr(inv_std),
+                                       ptr(dgamma), ptr(dbeta), ptr(dx), images, channels, pixels, groups, act, ptr(ws),
+                                       nbytes, stream_ptr()), "gn_backward")
+    return dgamma, dbeta, dx
+
+
+@_on_its_device
+def dropout(x, rate, seed, offset=0):
+    """``x`` with each element dropped (set to 0) with probability ``rate``, in steps of 2^-16, and the others divided by
+    the probability that they are kept.  The mask is a function of ``seed``, ``offset`` (64 bits each) and the element's index
+    alone and is stored nowhere: ``dropout_backward`` with the same numbers draws it again.  ``offset`` may be an int64
+    tensor of one element on the GPU: then a captured graph draws another mask whenever that number has changed."""
+    dtype = _dtype_of(x)
+    if not 0 <= rate <= 1:
+        raise ValueError(f"the rate of dropout is {rate}, it has to be between 0 and 1")
+    offset_dev = None
+    if isinstance(offset, torch.Tensor):
+        if offset.dtype != torch.int64 or offset.numel() != 1:
+            raise TypeError("the offset of dropout is a number or an int64 tensor of one element")
+        if offset.device != x.device:
+            raise ValueError(f"the offset is on {offset.device}, the tensor on {x.device}")
+        offset, offset_dev = 0, ptr(offset)
+    x = x.contiguous()
+    y = torch.empty_like(x)
+    if x.numel():
+        mask = (1 << 64) - 1
+        check(lib().pydtnn_hip_dropout(dtype, ptr(x), ptr(y), x.numel(), float(rate), int(seed) & mask, int(offset) & mask,
+                                       offset_dev, stream_ptr()), "dropout")
+    return y
+
+
+def dropout_backward(dy, rate, seed, offset=0):
+    """The gradient of ``dropout`` called with the same numbers: dy through the same mask."""
+    return dropout(dy, rate, seed, offset)

@@ -1,0 +1,147 @@
+"""CPU-side checks of the operators for several element types: the oracles against published values and differences, and
+what the entry points refuse (nothing here launches a kernel)."""
+import ctypes
+import os
+
+import numpy as np
+import pytest
+import torch
+
+import operator_oracles as oo
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from pydtnn_amd import native
+    if not os.path.exists(native.LIB_PATH):
+        import __graft_entry__
+        __graft_entry__.build()
+    return native.lib()
+
+
+@pytest.fixture(scope="module")
+def ops(lib):
+    from pydtnn_amd import ops
+    return ops
+
+
+@pytest.mark.parametrize("counter,key,words", [
+    ((0, 0, 0, 0), (0, 0), (0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8)),
+    ((0xFFFFFFFF,) * 4, (0xFFFFFFFF,) * 2, (0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD)),
+    ((0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344), (0xA4093822, 0x299F31D0),
+     (0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1)),
+])
+def test_the_generator_gives_its_authors_known_answers(counter, key, words):
+    """The known answers that the authors of Philox4x32-10 publish for it."""
+    assert tuple(int(w[0]) for w in oo.philox4x32_10([[c] for c in counter], key)) == words
+
+
+@pytest.mark.parametrize("activation", ["", "silu"])
+@pytest.mark.parametrize("nhwc", [True, False])
+def test_the_group_norm_gradient_of_the_oracle_is_the_slope_of_its_forward(activation, nhwc):
+    rng = np.random.default_rng(3)
+    shape = (2, 3, 4, 6) if nhwc else (2, 6, 3, 4)
+    x, dy = rng.standard_normal(shape), rng.standard_normal(shape)
+    gamma, beta = rng.standard_normal(6), rng.standard_normal(6)
+
+    def loss(x, gamma, beta):
+        return (oo.gn_forward(x, gamma, beta, 3, 1e-5, activation, nhwc)[0] * dy).sum()
+
+    _, mean, inv_std = oo.gn_forward(x, gamma, beta, 3, 1e-5, activation, nhwc)
+    grads = oo.gn_backward(dy, x, gamma, beta, mean, inv_std, 3, activation, nhwc)
+    h = 1e-5
+    for which, grad in ((1, grads[0]), (2, grads[1]), (0, grads[2])):
+        for _ in range(4):
+            v = [np.zeros(shape), np.zeros(6), np.zeros(6)]
+            v[which] = rng.standard_normal(v[which].shape)
+            slope = (loss(x + h * v[0], gamma + h * v[1], beta + h * v[2]) -
+                     loss(x - h * v[0], gamma - h * v[1], beta - h * v[2])) / (2 * h)
+            # the third derivative's h^2 and the difference's rounding, 1e-16 |loss| / h
+            assert abs(slope - (grad * v[which]).sum()) < 1e-6
+
+
+FAKE = 4096      # an address that a call which refuses its arguments never touches
+
+
+def test_gn_refuses_extents_it_cannot_run(lib):
+    p = ctypes.c_void_p(FAKE)
+
+    def forward(dtype=0, images=2, channels=8, pixels=4, groups=2, eps=1e-5, act=0, x=p, nbytes=None):
+        need = lib.pydtnn_hip_gn_workspace_bytes(dtype, 1, 0, images, channels, pixels, groups)
+        return lib.pydtnn_hip_gn_forward(dtype, 1, x, p, p, p, p, p, images, channels, pixels, groups, eps, act, p,
+                                         need - 1 if nbytes else need, None)
+
+    assert forward(x=None) == 1
+    assert forward(images=0) == forward(pixels=0) == forward(channels=0) == forward(groups=0) == 1
+    assert forward(groups=3) == 1
+    assert forward(eps=-1.0) == forward(eps=float("nan")) == 1
+    assert forward(nbytes=-1) == 2
+    assert forward(dtype=9) in (1, 2) and forward(act=7) == 1
+    assert forward(pixels=(1 << 30) + 1) == 4
+    assert lib.pydtnn_hip_gn_backward(0, 1, p, p, p, p, p, p, p, None, p, 2, 8, 4, 2, 0, p, 1 << 20, None) == 1
+    assert lib.pydtnn_hip_gn_backward(0, 1, p, p, p, p, p, p, p, p, p, 2, 8, 4, 2, 0, p, 8, None) == 2
+
+
+def test_dropout_refuses_rates_and_types_it_does_not_know(lib):
+    p = ctypes.c_void_p(FAKE)
+    for rate in (-0.1, 1.1, float("nan")):
+        assert lib.pydtnn_hip_dropout(0, p, p, 8, rate, 1, 0, None, None) == 1
+    assert lib.pydtnn_hip_dropout(4, p, p, 8, 0.5, 1, 0, None, None) == 1
+    assert lib.pydtnn_hip_dropout(0, p, p, 0, 0.5, 1, 0, None, None) == 1
+    assert lib.pydtnn_hip_dropout(0, None, p, 8, 0.5, 1, 0, None, None) == 1
+    assert lib.pydtnn_hip_dropout(0, p, p, 1 << 45, 0.5, 1, 0, None, None) == 4
+
+
+def test_gn_checks_its_tensors(ops):
+    x, v, s = torch.ones(2, 3, 3, 8), torch.ones(8), torch.ones(2, 4)
+    with pytest.raises(ValueError):
+        ops.gn_forward(x, v, v, 4)                                  # not on the GPU
+    with pytest.raises(ValueError):
+        ops.gn_forward(x, v, v, 3)
+    with pytest.raises(ValueError):
+        ops.gn_forward(x, v, v, 0)
+    with pytest.raises(ValueError):
+        ops.gn_forward(x, v[:4], v, 4)
+    with pytest.raises(ValueError):
+        ops.gn_forward(x, v, v, 4, activation="tanh")
+    with pytest.raises(ValueError):
+        ops.gn_forward(x, v, v, 4, eps=-1e-5)
+    with pytest.raises(ValueError):
+        ops.gn_forward(v, v, v, 4)
+    with pytest.raises(ValueError):
+        ops.gn_forward(x[:, :0], v, v, 4)
+    with pytest.raises(TypeError):
+        ops.gn_forward(x.int(), v, v, 4)
+    with pytest.raises(TypeError):
+        ops.gn_forward(x.half(), v.half(), v, 4)
+    with pytest.raises(TypeError):
+        ops.gn_forward(x.double(), v, v, 4)
+    with pytest.raises(ValueError):
+        ops.gn_backward(x, x, v, v, s[:1], s, 4)
+    with pytest.raises(TypeError):
+        ops.gn_backward(x.half(), x, v, v, s, s, 4)
+    with pytest.raises(ValueError):
+        ops.gn_backward(x[:1], x, v, v, s, s, 4)
+
+
+def test_dropout_checks_its_arguments(ops):
+    x = torch.ones(8)
+    for rate in (-0.1, 1.5, float("nan")):
+        with pytest.raises(ValueError):
+            ops.dropout(x, rate, 1)
+    with pytest.raises(ValueError):
+        ops.dropout(x, 0.5, 1)                                      # not on the GPU
+    with pytest.raises(TypeError):
+        ops.dropout(x.int(), 0.5, 1)
+    with pytest.raises(TypeError):
+        ops.dropout(x, 0.5, 1, torch.zeros(1))
+    with pytest.raises(TypeError):
+        ops.dropout(x, 0.5, 1, torch.zeros(2, dtype=torch.int64))
+
+
+def test_a_dropout_layer_checks_its_seed():
+    import pydtnn_amd as pd
+    for seed in (-1, 1 << 32):
+        with pytest.raises(ValueError):
+            pd.Dropout(rate=0.5, seed=seed)
+    assert pd.Dropout(rate=0.5).seed is None
