@@ -474,6 +474,22 @@ int pydtnn_hip_gn_backward(int dtype, int nhwc, const void *dy, const void *x, c
 int pydtnn_hip_dropout(int dtype, const void *x, void *y, long total, double rate, uint64_t seed, uint64_t offset,
                        const int64_t *offset_dev, void *stream);
 
+/* Matrix product in 8-bit floating point (e4m3: 4 exponent bits, 3 mantissa bits, largest value 448, no infinity) with
+ * a scale for each block of 128 consecutive k of a row, for FC layers that serve.
+ *   pydtnn_hip_quantize_fp8: x (rows, k) -> q (rows, kp), kp = k to a multiple of 128, zeros behind k, and scales
+ *       (rows, words * 4), words = kp / 128 / 4 rounded up, one byte for a block: e + 127 for the scale 2^e, the smallest
+ *       power of two with max |x| <= 448 * 2^e, e in [-127, 127]; 127 behind the last block.  x * 2^-e is rounded to the
+ *       nearest e4m3 value, to even between two.  A block that holds an infinity or a NaN is NaN throughout, its scale 1.
+ *   pydtnn_hip_matmul_fp8: y (m, n) = relu?( dequantised(quantised(x)) * dequantised(w)^T + bias ) with x (m, k) quantised on
+ *       the way and wq (n, kp), wscales as pydtnn_hip_quantize_fp8 makes them of the (n, k) weights, once.  bias (n) is
+ *       float32 or NULL; sums are held in float32.
+ * x and y are float32, float16 or bfloat16 (`dtype`; PYDTNN_HIP_ERR_INVALID for float64).  q and the workspace are aligned to
+ * 16 bytes, scales to 4.  Extents are at most 2^30.  Workspace: pydtnn_hip_matmul_fp8_workspace_bytes(m, n, k). */
+int pydtnn_hip_quantize_fp8(int dtype, const void *x, long rows, long k, uint8_t *q, uint8_t *scales, void *stream);
+size_t pydtnn_hip_matmul_fp8_workspace_bytes(long m, long n, long k);
+int pydtnn_hip_matmul_fp8(int dtype, const void *x, long m, long k, const uint8_t *wq, const uint8_t *wscales, long n,
+                          const float *bias, int relu, void *y, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ------------------------------------------------------------------------------------------
  * Host-pointer compatibility flavour (exported by libconvGemm.so only).  Signatures are those
  * PyDTNN's ctypes shim calls (pydtnn/backends/cpu/libs/conv_gemm.py:91-92, :191-205, :234-248,

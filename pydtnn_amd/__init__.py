@@ -7,7 +7,7 @@ importing the layers works anywhere, running them needs the built library and a 
 """
 from .layers import (EVALUATE_MODE, TRAIN_MODE, UNSPECIFIED_MODE, AdditionBlock, AveragePool2D, BatchNormalization,
                      BatchNormalizationRelu, Conv2D, Conv2DBatchNormalization, Conv2DBatchNormalizationRelu,
-                     Conv2DRelu, Dropout, FC, Flatten, GroupNormalization, Input, Layer, MaxPool2D, Relu, Softmax)
+                     Conv2DRelu, Dropout, FC, FCFp8, Flatten, GroupNormalization, Input, Layer, MaxPool2D, Relu, Softmax)
 from .model import SGD, CategoricalCrossEntropy, Model
 from . import models, tracers
 from .best_of import BestOf

@@ -950,6 +950,41 @@ class Conv2DBatchNormalizationRelu(_FusedConv):
     _with_relu = True
 
 
+# --------------------------------------------------------------------------- FC in 8-bit floating point
+class FCFp8(FC, _FromParents):
+    """An FC layer that serves with e4m3 weights and activations, each scaled by blocks of 128 along the inputs (inference
+    only).  The fusion pass makes it of an FC layer and of the Relu behind that, with ``Model(enable_fp8_fc=True)``.  The
+    weights are quantised when they are set; a change in place of ``weights`` has to be followed by setting them again.
+    In weights files it goes by the name of the layer it was."""
+
+    canonical_name = "FC"
+
+    def __init__(self, from_parent):
+        weights = from_parent.weights
+        self._adopt(from_parent)
+        self.__dict__.pop("weights")
+        self.relu = False
+        self.weights = weights
+
+    @property
+    def weights(self):
+        return self._weights
+
+    @weights.setter
+    def weights(self, weights):
+        self._weights = weights
+        if weights is not None:
+            self.wq, self.wscales = ops.quantize_fp8(weights.reshape(-1, weights.shape[-1]).t())
+
+    def forward(self, x):
+        if self.model.mode == TRAIN_MODE:
+            raise RuntimeError("Fused layers cannot be used in training mode!")
+        return ops.matmul_fp8(x, self.wq, self.wscales, bias=self.biases if self.use_bias else None, relu=self.relu)
+
+    def backward(self, dy):
+        raise RuntimeError(f"Backward method of {self.__class__.__name__} should not be called")
+
+
 # --------------------------------------------------------------------------- residual block
 class AdditionBlock(Layer):
     """pydtnn/layers/abstract_block_layer.py:25-57 + pydtnn/backends/cpu/layers/addition_block_cpu.py:28-60:

@@ -52,6 +52,10 @@ _DEFAULTS = dict(
     enable_fused_conv_relu=False,
     enable_fused_conv_bn=False,
     enable_fused_conv_bn_relu=False,
+    # Not a reference flag.  The fusion pass also rewrites FC layers, with the Relu behind them, into layers that serve
+    # with e4m3 weights and activations scaled by blocks of 128 (FCFp8): a quarter of the bytes to read, at the accuracy of
+    # values of 3 mantissa bits.  float32 models only.
+    enable_fp8_fc=False,
     # Not a reference flag.  Inside train_batch a Relu layer of the top-level sequence is computed by the stores
     # of its neighbours (the convolution before it, the convolution or pooling layer after it) instead of by
     # two passes of its own.  Losses, gradients, masks and updated weights are bit-identical either way; what
@@ -87,6 +91,8 @@ class Model:
             if kwargs.get("enable_conv_gemm"):
                 raise ValueError("the implicit ConvGemm route is float32 only; a float64 model uses the explicit one")
             self.kwargs["enable_conv_gemm"] = False
+            if self.kwargs["enable_fp8_fc"]:
+                raise ValueError("FC layers in 8 bits are part of float32 models only")
         self.tracer = NullTracer()
         self.layers = []
         self.layer_id = _layer_id_generator()
@@ -146,14 +152,18 @@ class Model:
         return out
 
     # ------------------------------------------------------------------ fusion (pydtnn/model.py:294-349)
-    def apply_layer_fusion(self, bn_relu=None, conv_relu=None, conv_bn=None, conv_bn_relu=None):
-        """Rewrites [Conv2D, BatchNormalization, Relu] runs into fused inference layers.  Flags default to
-        the model's ``enable_fused_*`` settings.  As in the reference a convolution is only fused when its
-        installed forward is one the fused class implements (the ``cg`` variants, never ``i2c``)."""
+    def apply_layer_fusion(self, bn_relu=None, conv_relu=None, conv_bn=None, conv_bn_relu=None, fp8_fc=None):
+        """Rewrites [Conv2D, BatchNormalization, Relu] runs, and with ``fp8_fc`` [FC, Relu] runs, into fused inference
+        layers.  Flags default to the model's ``enable_fused_*`` and ``enable_fp8_fc`` settings.  As in the
+        reference a convolution is only fused when its installed forward is one the fused class implements (the
+        ``cg`` variants, never ``i2c``)."""
         bn_relu = self.enable_fused_bn_relu if bn_relu is None else bn_relu
         conv_relu = self.enable_fused_conv_relu if conv_relu is None else conv_relu
         conv_bn = self.enable_fused_conv_bn if conv_bn is None else conv_bn
         conv_bn_relu = self.enable_fused_conv_bn_relu if conv_bn_relu is None else conv_bn_relu
+        fp8_fc = self.enable_fp8_fc if fp8_fc is None else fp8_fc
+        if fp8_fc and self.dtype != torch.float32:
+            raise ValueError("FC layers in 8 bits are part of float32 models only")
 
         def fusable(conv, cls):
             # pydtnn/model.py:313, :330: the convolution's installed forward must be one the fused class has
@@ -188,6 +198,12 @@ class Model:
                         fused[-1].canonical_name == "BatchNormalization":
                     prev = fused.pop()
                     curr = L.BatchNormalizationRelu(from_parent=prev)
+                elif fp8_fc and type(curr) is L.FC:
+                    curr = L.FCFp8(from_parent=curr)
+                elif fp8_fc and len(fused) > 0 and curr.canonical_name == "Relu" and \
+                        type(fused[-1]) is L.FCFp8 and not fused[-1].relu:
+                    curr = fused.pop()
+                    curr.relu = True
                 fused.append(curr)
             return fused
 
@@ -201,7 +217,7 @@ class Model:
                     for p in layer.paths:
                         link_blocks(p)
 
-        if bn_relu or conv_relu or conv_bn or conv_bn_relu:
+        if bn_relu or conv_relu or conv_bn or conv_bn_relu or fp8_fc:
             self.layers = fuse(self.layers)
             self._fused = True
             if conv_relu or conv_bn or conv_bn_relu:

@@ -647,3 +647,60 @@ def dropout(x, rate, seed, offset=0):
 def dropout_backward(dy, rate, seed, offset=0):
     """The gradient of ``dropout`` called with the same numbers: dy through the same mask."""
     return dropout(dy, rate, seed, offset)
+
+
+def _fp8_shapes(rows, k):
+    """Shapes of the quantised values and of the scales of a (rows, k) matrix."""
+    blocks = -(-k // 128)
+    return (rows, blocks * 128), (rows, -(-blocks // 4) * 4)
+
+
+def _need_fp8_input(x):
+    dtype = _dtype_of(x)
+    if x.dtype == torch.float64:
+        raise TypeError("8-bit products take float32, float16 or bfloat16")
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"a (rows, k) matrix is expected, not a tensor of shape {tuple(x.shape)}")
+    return dtype
+
+
+@_on_its_device
+def quantize_fp8(x):
+    """A (rows, k) matrix in e4m3 with a scale for each block of 128 consecutive elements of a row -> (q, scales).  q is
+    (rows, k to a multiple of 128), zeros behind k; scales holds e + 127 for the scale 2^e of a block, the smallest that brings
+    the block within 448, the largest e4m3 value (rows, blocks to a multiple of 4, uint8).  A block with an infinity or a NaN
+    becomes NaN throughout."""
+    dtype = _need_fp8_input(x)
+    x = x.contiguous()
+    q_shape, scales_shape = _fp8_shapes(*x.shape)
+    q = torch.empty(q_shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty(scales_shape, dtype=torch.uint8, device=x.device)
+    if x.shape[0]:
+        check(lib().pydtnn_hip_quantize_fp8(dtype, ptr(x), x.shape[0], x.shape[1], ptr(q), ptr(scales), stream_ptr()),
+              "quantize_fp8")
+    return q, scales
+
+
+@_on_its_device
+def matmul_fp8(x, wq, wscales, bias=None, relu=False):
+    """``x @ w.T (+ bias, ReLU)`` in e4m3 for (m, k) activations, which are quantised on the way, and weights that
+    ``quantize_fp8`` has made of an (n, k) matrix once.  Sums are held in 32 bits, bias is float32, the result has the type of
+    ``x``."""
+    dtype = _need_fp8_input(x)
+    m, k = x.shape
+    if wq.dim() != 2 or wq.shape[0] < 1:
+        raise ValueError(f"quantised weights are an (n, k) matrix, not a tensor of shape {tuple(wq.shape)}")
+    n = wq.shape[0]
+    q_shape, scales_shape = _fp8_shapes(n, k)
+    _need_like(x, torch.float8_e4m3fn, weights=(wq, q_shape))
+    _need_like(x, torch.uint8, scales=(wscales, scales_shape))
+    if bias is not None:
+        _need_like(x, torch.float32, bias=(bias, (n,)))
+    x = x.contiguous()
+    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    if m:
+        nbytes = lib().pydtnn_hip_matmul_fp8_workspace_bytes(m, n, k)
+        ws = _scratch(nbytes, x)
+        check(lib().pydtnn_hip_matmul_fp8(dtype, ptr(x), m, k, ptr(wq), ptr(wscales), n, ptr(bias), int(relu), ptr(y), ptr(ws),
+                                          nbytes, stream_ptr()), "matmul_fp8")
+    return y

@@ -339,6 +339,134 @@ def test_calls_on_two_streams_at_once(ops):
             assert all(torch.equal(t, r) for t, r in zip(out, ref))
 
 
+# --------------------------------------------------------------------------- e4m3 with a scale for each block of 128
+FP8_DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def fp8_matrix(rows, k, dtype, seed, spread=True):
+    """Values whose size changes from block to block and from row to row, a block of zeros, values at the edges."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, k, generator=g)
+    if spread:
+        x *= torch.exp2(torch.randint(-6, 5, (rows, -(-k // 128)), generator=g).float()).repeat_interleave(128, 1)[:, :k]
+        x[0, :128] = 0
+        x[-1, 0] = 448.0                       # the largest e4m3 value: its block keeps scale 1 or above
+        x[-1, k // 2] = 2.0 ** -9
+    return x.to(dtype).cuda()
+
+
+@pytest.mark.parametrize("dtype", FP8_DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [(1, 1), (3, 127), (2, 128), (5, 129), (1, 511), (7, 512), (4, 513), (9, 2049), (33, 1000)],
+                         ids=str)
+def test_quantization_is_its_plain_form_bit_for_bit(ops, shape, dtype):
+    announce("quantize", shape, dtype)
+    x = fp8_matrix(*shape, dtype, sum(shape))
+    ref, e = oo.quantize_fp8(oo.host64(x))
+    for t in (x, misaligned(x), x.t().contiguous().t()):
+        q, scales = ops.quantize_fp8(t)
+        assert np.array_equal(oo.host64(q), ref)
+        got = scales.cpu().numpy().astype(np.int64) - 127
+        assert np.array_equal(got[:, :e.shape[1]], e) and np.all(got[:, e.shape[1]:] == 0)
+
+
+def test_quantization_of_the_smallest_and_largest_values(ops):
+    """Scales at both ends of their range, values that a scale's edge decides, and ties."""
+    announce("quantize edges")
+    f = torch.finfo(torch.float32)
+    rows = [448.0, 448.0 * (1 + 2 ** -23), 447.99997, 224.0, f.max, f.tiny, 2.0 ** -149, 448 * 2.0 ** -127, 1.0, 17.0, 19.0,
+            2.0 ** -10, 3 * 2.0 ** -10]
+    x = torch.zeros(len(rows), 256)
+    x[:, 0] = torch.tensor(rows, dtype=torch.float64).float()
+    x[:, 5] = -x[:, 0] / 16 * 1.0625
+    x[:, 130] = x[:, 0] * 0.3
+    q, scales = ops.quantize_fp8(x.cuda())
+    ref, e = oo.quantize_fp8(oo.host64(x))
+    assert np.array_equal(scales.cpu().numpy()[:, :2].astype(np.int64) - 127, e)
+    assert np.array_equal(oo.host64(q), ref)
+
+
+# (m, n, k): from one element to ragged extents, few rows, many rows, long k
+FP8_SHAPES = [(1, 1, 1), (1, 1000, 4096), (2, 10, 130), (3, 63, 128), (7, 257, 513), (16, 64, 2048), (17, 16, 127),
+              (16, 96, 25088), (31, 100, 384), (33, 130, 1000), (64, 256, 1024), (65, 31, 640), (100, 1003, 777),
+              (129, 257, 2049), (257, 511, 300), (300, 640, 512), (512, 512, 4096), (1025, 384, 256)]
+
+
+@pytest.mark.parametrize("dtype", FP8_DTYPES, ids=str)
+@pytest.mark.parametrize("shape", FP8_SHAPES, ids=str)
+def test_matmul_fp8(ops, shape, dtype):
+    m, n, k = shape
+    announce("matmul_fp8", shape, dtype)
+    # weights small enough that float16 holds the products of the widest blocks
+    x, w = fp8_matrix(m, k, dtype, m + k), fp8_matrix(n, k, torch.float32, n + k, spread=n % 2 == 0) * 2.0 ** -7
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(n)).cuda()
+    wq, ws = ops.quantize_fp8(w)
+    hq, he = oo.quantize_fp8(oo.host64(w))
+    for b, relu in ((bias, True), (None, False)):
+        y = ops.matmul_fp8(x, wq, ws, bias=b, relu=relu)
+        assert y.dtype == dtype
+        ref, bound = oo.matmul_fp8(oo.host64(x), hq, he, None if b is None else oo.host64(b), relu, dtype)
+        within(y, ref, bound, "y")
+        # all results together: half a step each at most, and a sum's error, which does not add up with one sign
+        if m * n >= 64:
+            assert np.linalg.norm(oo.host64(y) - ref) <= (oo.HALF_STEP[dtype] + 2.0 ** -13) * np.linalg.norm(ref)
+        assert torch.equal(y, ops.matmul_fp8(misaligned(x), wq, ws, bias=b, relu=relu))
+
+
+def test_matmul_fp8_keeps_what_is_not_a_number_in_its_row(ops):
+    announce("matmul_fp8 NaN")
+    for m in (5, 200):
+        x, w = fp8_matrix(m, 700, torch.float32, 1), fp8_matrix(40, 700, torch.float32, 2)
+        wq, ws = ops.quantize_fp8(w)
+        clean = ops.matmul_fp8(x, wq, ws)
+        x[1, 600], x[3, 0] = float("nan"), float("-inf")
+        y = ops.matmul_fp8(x, wq, ws)
+        assert torch.isnan(y[[1, 3]]).all()
+        rest = [i for i in range(m) if i not in (1, 3)]
+        assert torch.equal(y[rest], clean[rest])
+        w[7, 699] = float("inf")
+        y = ops.matmul_fp8(fp8_matrix(m, 700, torch.float32, 1), *ops.quantize_fp8(w))
+        assert torch.isnan(y[:, 7]).all() and torch.equal(y[:, :7], clean[:, :7]) and torch.equal(y[:, 8:], clean[:, 8:])
+
+
+def test_matmul_fp8_of_strided_rows_and_of_none(ops):
+    announce("matmul_fp8 strides")
+    x, w = fp8_matrix(24, 400, torch.bfloat16, 3), fp8_matrix(40, 200, torch.float32, 4)
+    wq, ws = ops.quantize_fp8(w)
+    assert torch.equal(ops.matmul_fp8(x[:, ::2], wq, ws), ops.matmul_fp8(x[:, ::2].contiguous(), wq, ws))
+    assert ops.matmul_fp8(x[:0, :200], wq, ws).shape == (0, 40)
+    with pytest.raises(ValueError):
+        ops.matmul_fp8(x[:, :200], wq.as_strided(wq.shape, (1, 40)), ws)
+
+
+def test_matmul_fp8_in_graphs_and_on_two_streams(ops):
+    announce("matmul_fp8 graphs")
+    cases = []
+    for m, n, k in ((16, 300, 9000), (3, 1000, 4096), (400, 300, 1000)):
+        x, w = fp8_matrix(m, k, torch.float32, m), fp8_matrix(n, k, torch.float32, n)
+        wq, ws = ops.quantize_fp8(w)
+        cases.append((x, wq, ws, ops.matmul_fp8(x, wq, ws, relu=True)))
+    torch.cuda.synchronize()
+    graphs = []
+    for x, wq, ws, _ in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, ops.matmul_fp8(x, wq, ws, relu=True)))
+        graphs[-1] = (graph, graphs[-1][1])
+    streams = [torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(4):
+        for graph, y in graphs:
+            y.zero_()
+        torch.cuda.synchronize()
+        eager = []
+        for stream, (graph, y), (x, wq, ws, ref) in zip(streams, graphs, cases):
+            with torch.cuda.stream(stream):
+                graph.replay()
+                eager.append(ops.matmul_fp8(x, wq, ws, relu=True))
+        torch.cuda.synchronize()
+        for (graph, y), e, (x, wq, ws, ref) in zip(graphs, eager, cases):
+            assert torch.equal(y, ref) and torch.equal(e, ref)
+
+
 # --------------------------------------------------------------------------- layers
 @pytest.mark.parametrize("fmt", ["NCHW", "NHWC"])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float64], ids=str)
@@ -391,3 +519,120 @@ def test_dropout_layer_with_a_seed(pd):
     assert torch.equal(layers[0].forward(x) != 0, masks[0])
     model.mode = pd.EVALUATE_MODE
     assert layers[0].forward(x) is x and layers[0].backward(x) is x
+
+
+def test_fc_in_8_bits_after_the_fusion_pass(pd):
+    announce("FC in 8 bits")
+    rng = np.random.default_rng(4)
+    model = pd.Model(enable_fp8_fc=True)
+    model.add(pd.Input(shape=(300,)))
+    model.add(pd.FC(shape=(70,), activation="relu"))
+    model.add(pd.FC(shape=(10,), use_bias=False, activation="softmax"))
+    model.layers[1].biases = torch.from_numpy(rng.standard_normal(70).astype(np.float32)).cuda()
+    stored = {}
+    model.load_store_path(model.layers, stored, "store")
+    x = torch.randn(9, 300, device="cuda")
+    y = model.evaluate_dataset_batch(x)
+    assert [type(layer).__name__ for layer in model.layers] == ["Input", "FCFp8", "FCFp8", "Softmax"]
+    cur = x
+    for layer in model.layers[1:3]:
+        out = layer.forward(cur)
+        hq, he = oo.quantize_fp8(oo.host64(layer.weights).T)
+        ref, bound = oo.matmul_fp8(oo.host64(cur), hq, he, oo.host64(layer.biases) if layer.use_bias else None, layer.relu,
+                                   torch.float32)
+        within(out, ref, bound, "FC")
+        cur = out
+    assert model.layers[1].relu and not model.layers[2].relu
+    assert torch.equal(model.layers[3].forward(cur), y)
+    again = {}
+    model.load_store_path(model.layers, again, "store")
+    assert sorted(again) == sorted(stored) and all(np.array_equal(again[k], stored[k]) for k in stored)
+    # weights that are loaded are quantised anew
+    model.load_store_path(model.layers, {k: v * 2 for k, v in stored.items()}, "load")
+    assert torch.equal(model.layers[2].forward(model.layers[1].forward(x)), 4 * cur)
+    with pytest.raises(RuntimeError):
+        model.train_batch(x, y, pd.CategoricalCrossEntropy(), pd.SGD())
+    with pytest.raises(RuntimeError):
+        model.layers[1].backward(y)
+
+
+@pytest.mark.parametrize("fmt", ["NCHW", "NHWC"])
+def test_a_network_is_trained_with_group_norm_and_dropout_and_served_in_8_bits(pd, fmt):
+    """One step of a network whose blocks are normalised by groups and whose head drops by a seed, against the same network
+    in float64 on the CPU with the oracle's masks and torch's gradients, and the network served in 8 bits afterwards."""
+    announce("network", fmt)
+    nhwc = fmt == "NHWC"
+    model = pd.Model(tensor_format=fmt, enable_fp8_fc=True)
+    model.add(pd.Input(shape=(12, 10, 3)))
+    model.add(pd.Conv2D(nfilters=16, filter_shape=(3, 3), padding=1, use_bias=False))      # 1
+    model.add(pd.GroupNormalization(groups=4, activation="silu"))                           # 2
+    model.add(pd.MaxPool2D(pool_shape=(2, 2), stride=2))                                    # 3
+    model.add(pd.Conv2D(nfilters=24, filter_shape=(3, 3), padding=1, use_bias=False))      # 4
+    model.add(pd.GroupNormalization(groups=8))                                              # 5
+    model.add(pd.Flatten())                                                                 # 6
+    model.add(pd.FC(shape=(40,)))                                                           # 7
+    model.add(pd.Dropout(rate=0.5, seed=31))                                                # 8
+    model.add(pd.FC(shape=(10,), activation="softmax"))                                     # 9, 10
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn((6, 12, 10, 3) if nhwc else (6, 3, 12, 10), generator=g)
+    labels = torch.randint(0, 10, (6,), generator=g)
+    target = torch.zeros(6, 10)
+    target[torch.arange(6), labels] = 1
+    layers = model.layers
+    names = [(i, v) for i in (1, 2, 4, 5, 7, 9) for v in layers[i].grad_vars]
+    before = {(i, v): getattr(layers[i], v).double().cpu().clone().requires_grad_() for i, v in names}
+    loss = model.train_batch(x.cuda(), target.cuda(), pd.CategoricalCrossEntropy(), pd.SGD(learning_rate=0.0))
+
+    def conv(t, w):
+        w = w.permute(3, 0, 1, 2) if nhwc else w
+        t = t.permute(0, 3, 1, 2) if nhwc else t
+        t = torch.nn.functional.conv2d(t, w, padding=1)
+        return t.permute(0, 2, 3, 1) if nhwc else t
+
+    def norm(t, i, groups):
+        t = t.permute(0, 3, 1, 2) if nhwc else t
+        t = torch.nn.functional.group_norm(t, groups, before[i, "gamma"], before[i, "beta"], 1e-5)
+        return t.permute(0, 2, 3, 1) if nhwc else t
+
+    t = torch.nn.functional.silu(norm(conv(x.double(), before[1, "weights"]), 2, 4))
+    t = torch.nn.functional.max_pool2d(t.permute(0, 3, 1, 2), 2).permute(0, 2, 3, 1) if nhwc else \
+        torch.nn.functional.max_pool2d(t, 2)
+    t = norm(conv(t, before[4, "weights"]), 5, 8).reshape(6, -1)
+    t = t @ before[7, "weights"] + before[7, "biases"]
+    t = t * oo.dropout(torch.ones(6, 40, dtype=torch.float64), 0.5, 31 + (layers[8].id << 32), 1)
+    t = t @ before[9, "weights"] + before[9, "biases"]
+    ref = torch.nn.functional.cross_entropy(t, labels)
+    ref.backward()
+    # float32 through nine layers: each a sum of at most 720 terms, far from cancelling, so a part in 10^4 of the
+    # largest gradient is over a thousand half steps
+    assert abs(float(loss) - float(ref)) < 1e-4 * float(ref)
+    for i, v in names:
+        got, want = getattr(layers[i], layers[i].grad_vars[v]).double().cpu(), before[i, v].grad
+        assert got.reshape(want.shape).sub(want).abs().max() < 1e-4 * want.abs().max(), (i, v)
+    plain = model.evaluate_batch(x.cuda())
+    served = model.evaluate_dataset_batch(x.cuda())
+    assert type(model.layers[7]).__name__ == type(model.layers[9]).__name__ == "FCFp8"
+    cur = x.cuda()
+    for layer in model.layers[1:]:
+        out = layer.forward(cur)
+        if type(layer).__name__ == "FCFp8":
+            hq, he = oo.quantize_fp8(oo.host64(layer.weights).T)
+            want, bound = oo.matmul_fp8(oo.host64(cur), hq, he, oo.host64(layer.biases), False, torch.float32)
+            within(out, want, bound, "FC")
+        cur = out
+    assert torch.equal(cur, served) and served.shape == plain.shape
+
+
+def test_builders_with_group_norm_and_seeded_dropout(pd):
+    announce("builders")
+    model = pd.Model(tensor_format="NHWC")
+    pd.models.create_resnet50_imagenet(model, stages=((16, 1, 1), (32, 1, 2)), classes=7, input_shape=(32, 32, 3), groups=4)
+    kinds = {type(layer).__name__ for layer in model.get_all_layers()}
+    assert "GroupNormalization" in kinds and "BatchNormalization" not in kinds
+    x = torch.randn(2, 32, 32, 3, device="cuda")
+    target = torch.eye(7, device="cuda")[:2].contiguous()
+    loss = model.train_batch(x, target, pd.CategoricalCrossEntropy(), pd.SGD())
+    assert torch.isfinite(loss)
+    for layer in model.get_all_layers():
+        if type(layer).__name__ == "GroupNormalization":
+            assert torch.isfinite(layer.dgamma).all() and layer.dgamma.abs().max() > 0

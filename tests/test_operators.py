@@ -145,3 +145,71 @@ def test_a_dropout_layer_checks_its_seed():
         with pytest.raises(ValueError):
             pd.Dropout(rate=0.5, seed=seed)
     assert pd.Dropout(rate=0.5).seed is None
+
+
+def test_e4m3_of_the_oracle_is_the_type_of_torch():
+    v = np.concatenate([np.linspace(-448, 448, 40001), np.linspace(-0.04, 0.04, 4001), 2.0 ** np.arange(-12, 9.0)])
+    v = v.astype(np.float32)
+    assert np.array_equal(oo.e4m3(v.astype(np.float64)), oo.host64(torch.from_numpy(v).to(torch.float8_e4m3fn)))
+
+
+def test_fp8_refuses_what_it_cannot_run(lib):
+    p = ctypes.c_void_p(FAKE)
+
+    def quantize(dtype=0, rows=4, k=200, x=p, q=p, s=p):
+        return lib.pydtnn_hip_quantize_fp8(dtype, x, rows, k, q, s, None)
+
+    assert quantize(x=None) == quantize(q=None) == quantize(s=None) == 1
+    assert quantize(rows=0) == quantize(k=0) == quantize(dtype=1) == quantize(dtype=7) == 1
+    assert quantize(q=ctypes.c_void_p(FAKE + 8)) == quantize(s=ctypes.c_void_p(FAKE + 2)) == 1
+    assert quantize(k=(1 << 30) + 1) == 4
+
+    def matmul(dtype=0, m=4, k=200, n=6, x=p, w=p, s=p, y=p, ws=p, short=0):
+        need = lib.pydtnn_hip_matmul_fp8_workspace_bytes(m, n, k)
+        return lib.pydtnn_hip_matmul_fp8(dtype, x, m, k, w, s, n, None, 0, y, ws, max(need - short, 0), None)
+
+    assert matmul(x=None) == matmul(w=None) == matmul(s=None) == matmul(y=None) == 1
+    assert matmul(m=0) == matmul(k=0) == matmul(n=0) == matmul(dtype=1) == 1
+    assert matmul(w=ctypes.c_void_p(FAKE + 8)) == 1
+    assert matmul(ws=None) == matmul(short=1) == matmul(ws=ctypes.c_void_p(FAKE + 4)) == 2
+    assert matmul(n=(1 << 30) + 1) == 4
+
+
+def test_fp8_checks_its_tensors(ops):
+    x, q, s = torch.ones(3, 200), torch.ones(6, 256).to(torch.float8_e4m3fn), torch.ones(6, 4, dtype=torch.uint8)
+    with pytest.raises(ValueError):
+        ops.quantize_fp8(x)                                         # not on the GPU
+    with pytest.raises(ValueError):
+        ops.matmul_fp8(x, q, s)
+    for bad in (x.double(), x.int()):
+        with pytest.raises(TypeError):
+            ops.quantize_fp8(bad)
+        with pytest.raises(TypeError):
+            ops.matmul_fp8(bad, q, s)
+    for bad in (x[0], x[:, :0], x[None]):
+        with pytest.raises(ValueError):
+            ops.quantize_fp8(bad)
+        with pytest.raises(ValueError):
+            ops.matmul_fp8(bad, q, s)
+    with pytest.raises(ValueError):
+        ops.matmul_fp8(x, q[:, :128], s)
+    with pytest.raises(ValueError):
+        ops.matmul_fp8(x, q, s[:, :2])
+    with pytest.raises(ValueError):
+        ops.matmul_fp8(x, q[0], s)
+    with pytest.raises(TypeError):
+        ops.matmul_fp8(x, q.float(), s)
+    with pytest.raises(TypeError):
+        ops.matmul_fp8(x, q, s.int())
+    with pytest.raises(TypeError):
+        ops.matmul_fp8(x, q, s, bias=torch.ones(6).half())
+    with pytest.raises(ValueError):
+        ops.matmul_fp8(x, q, s, bias=torch.ones(5))
+
+
+def test_a_float64_model_has_no_8_bit_layers():
+    import pydtnn_amd as pd
+    with pytest.raises(ValueError):
+        pd.Model(dtype="float64", enable_fp8_fc=True)
+    with pytest.raises(ValueError):
+        pd.Model(dtype="float64").apply_layer_fusion(fp8_fc=True)
