@@ -22,17 +22,23 @@ namespace {
 constexpr int kT = 256;
 constexpr int kWave = 64;
 constexpr int kWaves = kT / kWave;
+constexpr int kWholeWidth = 512;      // channels of a slab that one kernel holds at most
 
 enum { kIdentity = 0, kRelu = 1, kSilu = 2 };
 
-__device__ __forceinline__ float exp_of(float v) { return expf(v); }
-__device__ __forceinline__ double exp_of(double v) { return exp(v); }
+// 1 / (1 + e^-z).  In 32 bits through the hardware's 2^v and 1/v, each within a step: their errors and that of the product
+// -z log2(e) move the result by a few steps of 1 + |z|.
+__device__ __forceinline__ float sigmoid(float z)
+{
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f));
+}
+__device__ __forceinline__ double sigmoid(double z) { return 1.0 / (1.0 + exp(-z)); }
 
 template <int ACT, typename A>
 __device__ __forceinline__ A act(A z)
 {
     if (ACT == kRelu) return z > (A)0 ? z : (A)0;
-    if (ACT == kSilu) return z / ((A)1 + exp_of(-z));
+    if (ACT == kSilu) return z * sigmoid(z);
     return z;
 }
 
@@ -41,6 +47,14 @@ __device__ __forceinline__ A wave_sum(A v)
 {
 #pragma unroll
     for (int o = kWave / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+    return v;
+}
+
+// The sum over `lanes` consecutive lanes, a power of two, in each of them.
+template <typename A>
+__device__ __forceinline__ A lanes_sum(A v, int lanes)
+{
+    for (int o = lanes / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
     return v;
 }
 
@@ -60,6 +74,9 @@ struct GnLast {
     int slab_groups, width, slabs;     // groups and channels of a slab, slabs of an image
     int tx, rows;
     int splits, run;                   // runs of pixels of an image, pixels of a run
+    long pieces;                       // images * slabs * splits
+    int group_lanes, column_lanes;     // threads that join the sums of one group, of one channel: powers of two, a wave at most
+    FastDiv by_columns;                // by the columns that a group has in a row of threads (join_threads)
 };
 
 struct Place {
@@ -67,12 +84,12 @@ struct Place {
     int slab, split, p0, p1, tx, ty;
 };
 
-__device__ __forceinline__ Place place_of(const GnLast& g)
+__device__ __forceinline__ Place place_of(const GnLast& g, unsigned piece)
 {
     Place at;
-    const unsigned b = blockIdx.x, per = (unsigned)(g.slabs * g.splits);
-    at.image = b / per;
-    const unsigned r = b % per;
+    const unsigned per = (unsigned)(g.slabs * g.splits);
+    at.image = piece / per;
+    const unsigned r = piece % per;
     at.slab = r / g.splits;
     at.split = r % g.splits;
     at.p0 = at.split * g.run;
@@ -82,82 +99,217 @@ __device__ __forceinline__ Place place_of(const GnLast& g)
     return at;
 }
 
+// The second pass walks the pieces from the last to the first, so that what the first pass read last is read again while
+// the caches hold it; in eights, since eight consecutive workgroups go to the eight dies and a piece should find its die's
+// second-level cache again.  The grid is a multiple of eight; places behind the last piece do nothing.
+__device__ __forceinline__ unsigned piece_from_the_end(unsigned block, unsigned blocks)
+{
+    return (blocks / 8 - 1 - block / 8) * 8 + block % 8;
+}
+
+// Neighbouring slabs of an image share lines of memory where their rows are shorter than a line: they go to one die, whose
+// second-level cache joins them.  Consecutive workgroups go to the eight dies in turn, so a die's pieces are every eighth.
+__device__ __forceinline__ long piece_of_die(long pieces)
+{
+    return (long)(blockIdx.x % 8) * ((pieces + 7) / 8) + blockIdx.x / 8;
+}
+
+// What the second pass writes goes past the caches, and what the first pass reads does not wait for lines of it to be
+// written back: forward 64 x 56 x 56 x 256 in float32 126 -> 102 us, backward 215 -> 182.  (Where one kernel does it all there
+// is no first pass to spare: 103 us with plain stores, 112 with these.)
+template <typename T, int V>
+__device__ __forceinline__ void stream_out(Pack<T, V>* to, const Pack<T, V>& v)
+{
+    if constexpr (sizeof(T) * V == 16) {
+        typedef uint32_t quad __attribute__((ext_vector_type(4)));
+        __builtin_nontemporal_store(*reinterpret_cast<const quad*>(&v), reinterpret_cast<quad*>(to));
+    } else {
+        *to = v;
+    }
+}
+
+// Loads of this many pixels are in flight before the first is used.
+constexpr int kAhead = 4;
+
+// Calls f(value of x at pixel p, p) for every pixel p of the thread's run, with kAhead loads under way at once.
+template <typename P, typename F>
+__device__ __forceinline__ void each_pixel(const Place& at, int rows, const P* x, long step, F f)
+{
+    int p = at.p0 + at.ty;
+    for (; p + (kAhead - 1) * rows < at.p1; p += kAhead * rows) {
+        P v[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) v[u] = x[(p + u * rows) * step];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) f(v[u], p + u * rows);
+    }
+    for (; p < at.p1; p += rows) f(x[p * step], p);
+}
+
+template <typename P, typename F>
+__device__ __forceinline__ void each_pixel_of_two(const Place& at, int rows, const P* x, const P* y, long step, F f)
+{
+    int p = at.p0 + at.ty;
+    for (; p + (kAhead - 1) * rows < at.p1; p += kAhead * rows) {
+        P v[kAhead], w[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            v[u] = x[(p + u * rows) * step];
+            w[u] = y[(p + u * rows) * step];
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) f(v[u], w[u], p + u * rows);
+    }
+    for (; p < at.p1; p += rows) f(x[p * step], y[p * step], p);
+}
+
+// Moments of one thread's elements of each of V channels, from differences from its own first element.
+template <typename A, int V>
+struct ThreadMoments {
+    A first[V], s1[V], s2[V];
+    int n;
+
+    template <typename T>
+    __device__ __forceinline__ void add(const Pack<T, V>& v)
+    {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if (n == 0) first[j] = (A)v.v[j];
+            const A d = (A)v.v[j] - first[j];
+            s1[j] += d;
+            s2[j] += d * d;
+        }
+        ++n;
+    }
+};
+
+// Joins the threads' moments to those of the slab's groups: calls f(group of the slab, count, mean, sum of squared
+// differences) in one lane for each.  Where no pack straddles groups, a thread first joins its own V channels.
+template <int THREADS, int V, typename A, typename F>
+__device__ __forceinline__ void join_threads(const GnLast& g, const ThreadMoments<A, V>& t, F f)
+{
+    __shared__ A part_mean[THREADS * V], part_m2[THREADS * V];
+    __shared__ int part_n[THREADS];
+    const int unit = g.cg % V == 0 ? V : 1;      // channels of an entry
+    A mean[V], m2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const A m = t.n ? t.s1[j] / (A)t.n : (A)0;
+        mean[j] = t.n ? t.first[j] + m : (A)0;
+        m2[j] = t.n ? t.s2[j] - t.s1[j] * m : (A)0;
+    }
+    part_n[threadIdx.x] = t.n * unit;
+    if (unit == V) {
+        // around the first channel's mean, as above around the first element
+        A sum = (A)0, squares = (A)0, all = (A)0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const A d = mean[j] - mean[0];
+            sum += d;
+            squares += d * d;
+            all += m2[j];
+        }
+        part_mean[threadIdx.x] = mean[0] + sum / (A)V;
+        part_m2[threadIdx.x] = all + (A)t.n * (squares - sum * sum / (A)V);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            part_mean[threadIdx.x * V + j] = mean[j];
+            part_m2[threadIdx.x * V + j] = m2[j];
+        }
+    }
+    __syncthreads();
+    // a group's entries are every column of a slab that is one group, else columns k mine .. of each row
+    const int each = V / unit, columns = g.tx * each, mine = g.slab_groups == 1 ? columns : g.cg / unit;
+    const int lane = threadIdx.x & (g.group_lanes - 1);
+    for (int k = threadIdx.x / g.group_lanes; k < g.slab_groups; k += THREADS / g.group_lanes) {
+        const int entries = mine * g.rows;
+        double count = 0, sum = 0, squares = 0;
+        for (int e = lane; e < entries; e += g.group_lanes) {
+            const int row = (int)fd_div((uint32_t)e, g.by_columns), i = row * columns + k * mine + e - row * mine;
+            const double n = part_n[unit == V ? i : i / V];
+            count += n;
+            sum += n * (double)part_mean[i];
+        }
+        count = lanes_sum(count, g.group_lanes);
+        const double centre = lanes_sum(sum, g.group_lanes) / count;
+        for (int e = lane; e < entries; e += g.group_lanes) {
+            const int row = (int)fd_div((uint32_t)e, g.by_columns), i = row * columns + k * mine + e - row * mine;
+            const double d = (double)part_mean[i] - centre;
+            squares += part_n[unit == V ? i : i / V] * d * d + (double)part_m2[i];
+        }
+        squares = lanes_sum(squares, g.group_lanes);
+        if (lane == 0) f(k, count, centre, squares);
+    }
+}
+
 // The moments of each group's piece: partial[(image * groups + group) * splits + split].
 template <typename T, int V>
 __global__ void __launch_bounds__(kT) gn_last_moments(const T* __restrict__ x, Moments<wide_t<T>>* __restrict__ partial,
                                                       GnLast g)
 {
     using A = wide_t<T>;
-    __shared__ A part_mean[kT * V], part_m2[kT * V];
-    __shared__ int part_n[kT];
-    const Place at = place_of(g);
+    const Place at = place_of(g, blockIdx.x);
     const T* base = x + (at.image * g.pixels) * g.channels + at.slab * g.width;
-    // differences from the thread's own first value keep the sums small
-    A first[V], s1[V] = {}, s2[V] = {};
-    int n = 0;
+    ThreadMoments<A, V> t = {};
     if (at.ty < g.rows) {
-        for (int c = at.tx * V; c < g.width; c += g.tx * V) {
-            for (int p = at.p0 + at.ty; p < at.p1; p += g.rows) {
-                const Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(base + (long)p * g.channels + c);
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    if (n == 0) first[j] = (A)v.v[j];
-                    const A d = (A)v.v[j] - first[j];
-                    s1[j] += d;
-                    s2[j] += d * d;
-                }
-                ++n;
-            }
-        }
+        for (int c = at.tx * V; c < g.width; c += g.tx * V)
+            each_pixel(at, g.rows, reinterpret_cast<const Pack<T, V>*>(base + c), g.channels / V,
+                       [&](const Pack<T, V>& v, int) { t.add(v); });
     }
-    part_n[threadIdx.x] = n;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const A m = n ? s1[j] / (A)n : (A)0;
-        part_mean[threadIdx.x * V + j] = n ? first[j] + m : (A)0;
-        part_m2[threadIdx.x * V + j] = n ? s2[j] - s1[j] * m : (A)0;
-    }
-    __syncthreads();
-    // a group's channels are every column of a slab that is one group, else columns k cg .. of each row
-    const int columns = g.tx * V, mine = g.slab_groups == 1 ? columns : g.cg;
-    for (int k = threadIdx.x / kWave; k < g.slab_groups; k += kWaves) {
-        const int entries = mine * g.rows;
-        double count = 0, sum = 0, m2 = 0;
-        for (int e = threadIdx.x % kWave; e < entries; e += kWave) {
-            const int i = (e / mine) * columns + k * mine + e % mine;
-            count += part_n[i / V];
-            sum += part_n[i / V] * (double)part_mean[i];
-        }
-        count = wave_sum(count);
-        const double mean = wave_sum(sum) / count;
-        for (int e = threadIdx.x % kWave; e < entries; e += kWave) {
-            const int i = (e / mine) * columns + k * mine + e % mine;
-            const double d = (double)part_mean[i] - mean;
-            m2 += part_n[i / V] * d * d + (double)part_m2[i];
-        }
-        m2 = wave_sum(m2);
-        if (threadIdx.x % kWave == 0) {
-            const long group = at.image * g.groups + at.slab * g.slab_groups + k;
-            partial[group * g.splits + at.split] = Moments<A>{(A)mean, (A)m2};
-        }
-    }
+    join_threads<kT>(g, t, [&](int k, double, double mean, double m2) {
+        const long group = at.image * g.groups + at.slab * g.slab_groups + k;
+        partial[group * g.splits + at.split] = Moments<A>{(A)mean, (A)m2};
+    });
 }
 
-// Mean and 1/std of one group from the moments of its pieces, `run_of(i)` elements each.
+// Mean and 1/std of one group from the moments of its pieces, `run_of(i)` elements each, by `lanes` consecutive threads;
+// all of them get the results.
 template <typename A, typename F>
-__device__ __forceinline__ void join_moments(const Moments<A>* part, int pieces, F run_of, double m, double eps, A* mean_out,
-                                             A* inv_std_out)
+__device__ __forceinline__ void join_moments(const Moments<A>* part, int pieces, F run_of, double m, double eps, int lanes,
+                                             A* mean_out, A* inv_std_out)
 {
+    const int lane = threadIdx.x & (lanes - 1);
     double sum = 0, m2 = 0;
-    for (int i = 0; i < pieces; ++i) sum += run_of(i) * (double)part[i].mean;
-    const double mean = sum / m;
-    for (int i = 0; i < pieces; ++i) {
+#pragma unroll 4
+    for (int i = lane; i < pieces; i += lanes) sum += run_of(i) * (double)part[i].mean;
+    const double mean = lanes_sum(sum, lanes) / m;
+#pragma unroll 4
+    for (int i = lane; i < pieces; i += lanes) {
         const double d = (double)part[i].mean - mean;
         m2 += run_of(i) * d * d + (double)part[i].m2;
     }
+    m2 = lanes_sum(m2, lanes);
     *mean_out = (A)mean;
     *inv_std_out = (A)(1.0 / sqrt(m2 / m + eps));
 }
+
+// y = act((x - mean) scale + shift) of V channels.
+template <typename A, int V>
+struct ChanFwd {
+    A mean[V], scale[V], shift[V];
+
+    // channels c .. of the slab, whose groups' statistics are given
+    __device__ __forceinline__ void set(const GnLast& g, int slab, int c, const A* group_mean, const A* group_inv_std,
+                                        const A* gamma, const A* beta)
+    {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int k = (c + j) / g.cg, ch = slab * g.width + c + j;
+            mean[j] = group_mean[k];
+            scale[j] = group_inv_std[k] * gamma[ch];
+            shift[j] = beta[ch];
+        }
+    }
+
+    template <int ACT, typename T>
+    __device__ __forceinline__ Pack<T, V> apply(Pack<T, V> v) const
+    {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v.v[j] = (T)act<ACT>(((A)v.v[j] - mean[j]) * scale[j] + shift[j]);
+        return v;
+    }
+};
 
 template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(kT) gn_last_apply(const T* __restrict__ x, const wide_t<T>* __restrict__ gamma,
@@ -168,37 +320,73 @@ __global__ void __launch_bounds__(kT) gn_last_apply(const T* __restrict__ x, con
 {
     using A = wide_t<T>;
     __shared__ A mean[kT * V], inv_std[kT * V];      // of the slab's groups: at most a group to a column
-    const Place at = place_of(g);
-    for (int k = threadIdx.x; k < g.slab_groups; k += kT) {
+    const unsigned piece = piece_from_the_end(blockIdx.x, gridDim.x);
+    if (piece >= g.pieces) return;
+    const Place at = place_of(g, piece);
+    for (int k = threadIdx.x / g.group_lanes; k < g.slab_groups; k += kT / g.group_lanes) {
         const long group = at.image * g.groups + at.slab * g.slab_groups + k;
+        A m, r;
         join_moments<A>(partial + group * g.splits, g.splits,
                         [&](int i) { return (double)(min(g.run, g.pixels - i * g.run)) * g.cg; },
-                        (double)g.pixels * g.cg, eps, &mean[k], &inv_std[k]);
-        if (at.split == 0) {
-            mean_out[group] = mean[k];
-            inv_std_out[group] = inv_std[k];
+                        (double)g.pixels * g.cg, eps, g.group_lanes, &m, &r);
+        if (threadIdx.x % g.group_lanes == 0) {
+            mean[k] = m;
+            inv_std[k] = r;
+            if (at.split == 0) {
+                mean_out[group] = m;
+                inv_std_out[group] = r;
+            }
         }
     }
     __syncthreads();
     if (at.ty >= g.rows) return;
     const long base = (at.image * g.pixels) * g.channels + at.slab * g.width;
     for (int c = at.tx * V; c < g.width; c += g.tx * V) {
-        A mu[V], scale[V], shift[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int k = (c + j) / g.cg, ch = at.slab * g.width + c + j;
-            mu[j] = mean[k];
-            scale[j] = inv_std[k] * gamma[ch];
-            shift[j] = beta[ch];
-        }
-        for (int p = at.p0 + at.ty; p < at.p1; p += g.rows) {
-            const long i = base + (long)p * g.channels + c;
-            Pack<T, V> v = *reinterpret_cast<const Pack<T, V>*>(x + i);
-#pragma unroll
-            for (int j = 0; j < V; ++j) v.v[j] = (T)act<ACT>(((A)v.v[j] - mu[j]) * scale[j] + shift[j]);
-            *reinterpret_cast<Pack<T, V>*>(y + i) = v;
-        }
+        ChanFwd<A, V> ch;
+        ch.set(g, at.slab, c, mean, inv_std, gamma, beta);
+        const long step = -(g.channels / V), from = base + c + (long)(at.p0 + at.p1 - 1) * g.channels;
+        Pack<T, V>* out = reinterpret_cast<Pack<T, V>*>(y + from);
+        each_pixel(at, g.rows, reinterpret_cast<const Pack<T, V>*>(x + from), step,
+                   [&](const Pack<T, V>& v, int p) { stream_out(out + p * step, ch.template apply<ACT>(v)); });
     }
+}
+
+// Both steps in one kernel where the registers of a workgroup hold a slab of an image: x is read once.
+template <typename T, int V, int ACT, int THREADS, int PACKS>
+__global__ void __launch_bounds__(THREADS) gn_last_whole(const T* __restrict__ x, const wide_t<T>* __restrict__ gamma,
+                                                         const wide_t<T>* __restrict__ beta, T* __restrict__ y,
+                                                         wide_t<T>* __restrict__ mean_out,
+                                                         wide_t<T>* __restrict__ inv_std_out, double eps, GnLast g)
+{
+    using A = wide_t<T>;
+    __shared__ A mean[kWholeWidth], inv_std[kWholeWidth];
+    const long piece = piece_of_die(g.pieces);
+    if (piece >= g.pieces) return;
+    const Place at = place_of(g, (unsigned)piece);
+    const long step = g.channels / V, base = (at.image * g.pixels) * g.channels + at.slab * g.width + at.tx * V;
+    const Pack<T, V>* in = reinterpret_cast<const Pack<T, V>*>(x + base);
+    Pack<T, V>* out = reinterpret_cast<Pack<T, V>*>(y + base);
+    const int mine = at.ty < g.rows ? (g.pixels - at.ty + g.rows - 1) / g.rows : 0;      // pixels of this thread
+    Pack<T, V> v[PACKS];
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i)
+        if (i < mine) v[i] = in[(at.ty + i * g.rows) * step];
+    ThreadMoments<A, V> t = {};
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i)
+        if (i < mine) t.add(v[i]);
+    join_threads<THREADS>(g, t, [&](int k, double count, double m, double m2) {
+        const long group = at.image * g.groups + at.slab * g.slab_groups + k;
+        mean_out[group] = mean[k] = (A)m;
+        inv_std_out[group] = inv_std[k] = (A)(1.0 / sqrt(m2 / count + eps));
+    });
+    __syncthreads();
+    if (!mine) return;
+    ChanFwd<A, V> ch;
+    ch.set(g, at.slab, at.tx * V, mean, inv_std, gamma, beta);
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i)
+        if (i < mine) out[(at.ty + i * g.rows) * step] = ch.template apply<ACT>(v[i]);
 }
 
 // What the backward pass needs of a channel of an image to compute dz from x and dy.
@@ -239,7 +427,7 @@ __device__ __forceinline__ A dz_of(const ChanBwd<A>& c, A x, A xn, A dy)
 {
     if (ACT == kRelu) return x * c.sign > c.border ? dy : (A)0;
     if (ACT == kSilu) {
-        const A z = xn * c.gamma + c.beta, p = (A)1 / ((A)1 + exp_of(-z));
+        const A z = xn * c.gamma + c.beta, p = sigmoid(z);
         return dy * (p * ((A)1 + z * ((A)1 - p)));
     }
     return dy;
@@ -254,6 +442,73 @@ __device__ __forceinline__ A dx_of(const ChanBwd<A>& c, A xn, A dz, A a, A b)
     return c.inv_std * ((g - a) - xn * b);
 }
 
+// V channels of an image: their constants, sums of dz and dz xn, and dx.
+template <typename A, int V>
+struct ChansBwd {
+    ChanBwd<A> ch[V];
+
+    template <int ACT>
+    __device__ __forceinline__ void set(const GnLast& g, long image, int channel, const A* mean, const A* inv_std,
+                                        const A* gamma, const A* beta)
+    {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const long group = image * g.groups + (channel + j) / g.cg;
+            ch[j] = chan_bwd<ACT>(mean[group], inv_std[group], gamma[channel + j], beta[channel + j]);
+        }
+    }
+
+    template <int ACT, typename T>
+    __device__ __forceinline__ void add(const Pack<T, V>& x, const Pack<T, V>& dy, A* s1, A* s2) const
+    {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const A xn = ((A)x.v[j] - ch[j].mean) * ch[j].inv_std;
+            const A dz = dz_of<ACT>(ch[j], (A)x.v[j], xn, (A)dy.v[j]);
+            s1[j] += dz;
+            s2[j] += dz * xn;
+        }
+    }
+
+    template <int ACT, typename T>
+    __device__ __forceinline__ Pack<T, V> apply(const Pack<T, V>& x, Pack<T, V> dy, const A* a, const A* b) const
+    {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const A xn = ((A)x.v[j] - ch[j].mean) * ch[j].inv_std;
+            const A dz = dz_of<ACT>(ch[j], (A)x.v[j], xn, (A)dy.v[j]);
+            dy.v[j] = (T)dx_of(ch[j], xn, dz, a[j], b[j]);
+        }
+        return dy;
+    }
+};
+
+// Sums of a run's dz and dz xn in each of the slab's channels c0 .. c0 + columns: f(channel of the slab, the two sums).
+template <int THREADS, int V, typename A, typename F>
+__device__ __forceinline__ void join_rows(const GnLast& g, int c0, const A* s1, const A* s2, F f)
+{
+    __shared__ A part1[THREADS * V], part2[THREADS * V];
+    const int columns = g.tx * V;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        part1[threadIdx.x * V + j] = s1[j];
+        part2[threadIdx.x * V + j] = s2[j];
+    }
+    __syncthreads();
+    const int lane = threadIdx.x & (g.column_lanes - 1);
+    for (int i = threadIdx.x / g.column_lanes; i < min(columns, g.width - c0); i += THREADS / g.column_lanes) {
+        A t1 = (A)0, t2 = (A)0;
+        for (int r = lane; r < g.rows; r += g.column_lanes) {
+            t1 += part1[r * columns + i];
+            t2 += part2[r * columns + i];
+        }
+        t1 = lanes_sum(t1, g.column_lanes);
+        t2 = lanes_sum(t2, g.column_lanes);
+        if (lane == 0) f(c0 + i, t1, t2);
+    }
+}
+
 // Sums of dz and dz xn over a run's pixels: sums[(image * splits + split) * channels + channel], then the same of dz xn.
 template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(kT) gn_last_bwd_sums(const T* __restrict__ dy, const T* __restrict__ x,
@@ -264,91 +519,192 @@ __global__ void __launch_bounds__(kT) gn_last_bwd_sums(const T* __restrict__ dy,
                                                        wide_t<T>* __restrict__ sums, GnLast g)
 {
     using A = wide_t<T>;
-    __shared__ A part1[kT * V], part2[kT * V];
-    const Place at = place_of(g);
+    const Place at = place_of(g, blockIdx.x);
     const long base = (at.image * g.pixels) * g.channels + at.slab * g.width;
     A* out1 = sums + (at.image * g.splits + at.split) * g.channels + at.slab * g.width;
     A* out2 = out1 + g.images * g.splits * g.channels;
-    const int columns = g.tx * V;
-    for (int c0 = 0; c0 < g.width; c0 += columns) {
+    for (int c0 = 0; c0 < g.width; c0 += g.tx * V) {
         const int c = c0 + at.tx * V;
         A s1[V] = {}, s2[V] = {};
         if (at.ty < g.rows && c < g.width) {
-            ChanBwd<A> ch[V];
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const int i = at.slab * g.width + c + j;
-                const long group = at.image * g.groups + i / g.cg;
-                ch[j] = chan_bwd<ACT>(mean[group], inv_std[group], gamma[i], beta[i]);
-            }
-            for (int p = at.p0 + at.ty; p < at.p1; p += g.rows) {
-                const long i = base + (long)p * g.channels + c;
-                const Pack<T, V> xv = *reinterpret_cast<const Pack<T, V>*>(x + i);
-                const Pack<T, V> dv = *reinterpret_cast<const Pack<T, V>*>(dy + i);
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const A xn = ((A)xv.v[j] - ch[j].mean) * ch[j].inv_std;
-                    const A dz = dz_of<ACT>(ch[j], (A)xv.v[j], xn, (A)dv.v[j]);
-                    s1[j] += dz;
-                    s2[j] += dz * xn;
-                }
-            }
+            ChansBwd<A, V> ch;
+            ch.template set<ACT>(g, at.image, at.slab * g.width + c, mean, inv_std, gamma, beta);
+            each_pixel_of_two(at, g.rows, reinterpret_cast<const Pack<T, V>*>(x + base + c),
+                              reinterpret_cast<const Pack<T, V>*>(dy + base + c), g.channels / V,
+                              [&](const Pack<T, V>& xv, const Pack<T, V>& dv, int) { ch.template add<ACT>(xv, dv, s1, s2); });
         }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            part1[threadIdx.x * V + j] = s1[j];
-            part2[threadIdx.x * V + j] = s2[j];
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < min(columns, g.width - c0); i += kT) {
-            A t1 = (A)0, t2 = (A)0;
-            for (int r = 0; r < g.rows; ++r) {
-                t1 += part1[r * columns + i];
-                t2 += part2[r * columns + i];
-            }
-            out1[c0 + i] = t1;
-            out2[c0 + i] = t2;
-        }
-        __syncthreads();
+        join_rows<kT, V>(g, c0, s1, s2, [&](int i, A t1, A t2) {
+            out1[i] = t1;
+            out2[i] = t2;
+        });
     }
 }
 
+// dgamma and dbeta of kParamChannels channels: the channel sums over images and runs, kParamRows threads a channel.
+constexpr int kParamChannels = 4, kParamRows = kT / kParamChannels;
+
+template <typename A>
+__device__ __forceinline__ void bwd_params(const A* __restrict__ sums, A* __restrict__ dgamma, A* __restrict__ dbeta,
+                                           long pieces, int channels, int block)
+{
+    __shared__ double part1[kT], part2[kT];
+    const int c = block * kParamChannels + threadIdx.x % kParamChannels, r = threadIdx.x / kParamChannels;
+    double t1 = 0, t2 = 0;
+    if (c < channels) {
+#pragma unroll 4
+        for (long i = r; i < pieces; i += kParamRows) {
+            t1 += (double)sums[i * channels + c];
+            t2 += (double)sums[(pieces + i) * channels + c];
+        }
+    }
+    part1[threadIdx.x] = t1;
+    part2[threadIdx.x] = t2;
+    __syncthreads();
+    for (int half = kParamRows / 2; half > 0; half /= 2) {
+        if (r < half) {
+            part1[threadIdx.x] += part1[threadIdx.x + half * kParamChannels];
+            part2[threadIdx.x] += part2[threadIdx.x + half * kParamChannels];
+        }
+        __syncthreads();
+    }
+    if (r == 0 && c < channels) {
+        dbeta[c] = (A)part1[threadIdx.x];
+        dgamma[c] = (A)part2[threadIdx.x];
+    }
+}
+
+template <typename A>
+__global__ void __launch_bounds__(kT) gn_bwd_params(const A* __restrict__ sums, A* __restrict__ dgamma,
+                                                    A* __restrict__ dbeta, long pieces, int channels)
+{
+    bwd_params(sums, dgamma, dbeta, pieces, channels, blockIdx.x);
+}
+
+// A and B of one group from the channel sums of its runs, by `lanes` consecutive threads.
+template <typename A>
+__device__ __forceinline__ void group_ab(const A* s1, const A* s2, const A* gamma, int c0, int cg, int splits, int channels,
+                                         double m, int lanes, A* a_out, A* b_out)
+{
+    double a = 0, b = 0;
+    const int lane = threadIdx.x & (lanes - 1);
+    for (int c = c0 + lane; c < c0 + cg; c += lanes) {
+#pragma unroll 4
+        for (int s = 0; s < splits; ++s) {
+            const long at = (long)s * channels + c;
+            a += (double)s1[at] * (double)gamma[c];
+            b += (double)s2[at] * (double)gamma[c];
+        }
+    }
+    a = lanes_sum(a, lanes);
+    b = lanes_sum(b, lanes);
+    if (lane == 0) {
+        *a_out = (A)(a / m);
+        *b_out = (A)(b / m);
+    }
+}
+
+// dx, and in the first workgroups dgamma and dbeta.
 template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(kT) gn_last_bwd_apply(const T* __restrict__ dy, const T* __restrict__ x,
                                                         const wide_t<T>* __restrict__ gamma,
                                                         const wide_t<T>* __restrict__ beta,
                                                         const wide_t<T>* __restrict__ mean,
                                                         const wide_t<T>* __restrict__ inv_std,
-                                                        const wide_t<T>* __restrict__ ab, T* __restrict__ dx, GnLast g)
+                                                        const wide_t<T>* __restrict__ sums, wide_t<T>* __restrict__ dgamma,
+                                                        wide_t<T>* __restrict__ dbeta, T* __restrict__ dx, int param_blocks,
+                                                        GnLast g)
 {
     using A = wide_t<T>;
-    const Place at = place_of(g);
+    __shared__ A group_a[kT * V], group_b[kT * V];
+    if ((int)blockIdx.x < param_blocks) {
+        if ((int)blockIdx.x * kParamChannels < g.channels)
+            bwd_params(sums, dgamma, dbeta, g.images * g.splits, g.channels, blockIdx.x);
+        return;
+    }
+    const unsigned piece = piece_from_the_end(blockIdx.x - param_blocks, gridDim.x - param_blocks);
+    if (piece >= g.pieces) return;
+    const Place at = place_of(g, piece);
+    const A* s1 = sums + at.image * g.splits * g.channels;
+    for (int k = threadIdx.x / g.group_lanes; k < g.slab_groups; k += kT / g.group_lanes)
+        group_ab(s1, s1 + g.images * g.splits * g.channels, gamma, at.slab * g.width + k * g.cg, g.cg, g.splits, g.channels,
+                 (double)g.cg * g.pixels, g.group_lanes, &group_a[k], &group_b[k]);
+    __syncthreads();
     if (at.ty >= g.rows) return;
     const long base = (at.image * g.pixels) * g.channels + at.slab * g.width;
     for (int c = at.tx * V; c < g.width; c += g.tx * V) {
-        ChanBwd<A> ch[V];
+        ChansBwd<A, V> ch;
+        ch.template set<ACT>(g, at.image, at.slab * g.width + c, mean, inv_std, gamma, beta);
         A a[V], b[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const int i = at.slab * g.width + c + j;
-            const long group = at.image * g.groups + i / g.cg;
-            ch[j] = chan_bwd<ACT>(mean[group], inv_std[group], gamma[i], beta[i]);
-            a[j] = ab[2 * group];
-            b[j] = ab[2 * group + 1];
+            a[j] = group_a[(c + j) / g.cg];
+            b[j] = group_b[(c + j) / g.cg];
         }
-        for (int p = at.p0 + at.ty; p < at.p1; p += g.rows) {
-            const long i = base + (long)p * g.channels + c;
-            const Pack<T, V> xv = *reinterpret_cast<const Pack<T, V>*>(x + i);
-            Pack<T, V> dv = *reinterpret_cast<const Pack<T, V>*>(dy + i);
+        const long step = -(g.channels / V), from = base + c + (long)(at.p0 + at.p1 - 1) * g.channels;
+        Pack<T, V>* out = reinterpret_cast<Pack<T, V>*>(dx + from);
+        each_pixel_of_two(at, g.rows, reinterpret_cast<const Pack<T, V>*>(x + from),
+                          reinterpret_cast<const Pack<T, V>*>(dy + from), step,
+                          [&](const Pack<T, V>& xv, const Pack<T, V>& dv, int p) {
+                              stream_out(out + p * step, ch.template apply<ACT>(xv, dv, a, b));
+                          });
+    }
+}
+
+// Sums and dx in one kernel where the registers of a workgroup hold a slab of an image of x and of dy: both are read once.
+template <typename T, int V, int ACT, int THREADS, int PACKS>
+__global__ void __launch_bounds__(THREADS) gn_last_bwd_whole(const T* __restrict__ dy, const T* __restrict__ x,
+                                                             const wide_t<T>* __restrict__ gamma,
+                                                             const wide_t<T>* __restrict__ beta,
+                                                             const wide_t<T>* __restrict__ mean,
+                                                             const wide_t<T>* __restrict__ inv_std,
+                                                             wide_t<T>* __restrict__ sums, T* __restrict__ dx, GnLast g)
+{
+    using A = wide_t<T>;
+    __shared__ A group_a[kWholeWidth], group_b[kWholeWidth], chan1[kWholeWidth], chan2[kWholeWidth];
+    const long piece = piece_of_die(g.pieces);
+    if (piece >= g.pieces) return;
+    const Place at = place_of(g, (unsigned)piece);
+    const long step = g.channels / V, base = (at.image * g.pixels) * g.channels + at.slab * g.width + at.tx * V;
+    const Pack<T, V>* xin = reinterpret_cast<const Pack<T, V>*>(x + base);
+    const Pack<T, V>* din = reinterpret_cast<const Pack<T, V>*>(dy + base);
+    Pack<T, V>* out = reinterpret_cast<Pack<T, V>*>(dx + base);
+    const int mine = at.ty < g.rows ? (g.pixels - at.ty + g.rows - 1) / g.rows : 0;      // pixels of this thread
+    Pack<T, V> xv[PACKS], dv[PACKS];
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const A xn = ((A)xv.v[j] - ch[j].mean) * ch[j].inv_std;
-                const A dz = dz_of<ACT>(ch[j], (A)xv.v[j], xn, (A)dv.v[j]);
-                dv.v[j] = (T)dx_of(ch[j], xn, dz, a[j], b[j]);
-            }
-            *reinterpret_cast<Pack<T, V>*>(dx + i) = dv;
+    for (int i = 0; i < PACKS; ++i) {
+        if (i < mine) {
+            xv[i] = xin[(at.ty + i * g.rows) * step];
+            dv[i] = din[(at.ty + i * g.rows) * step];
         }
     }
+    ChansBwd<A, V> ch;
+    A s1[V] = {}, s2[V] = {};
+    if (mine) ch.template set<ACT>(g, at.image, at.slab * g.width + at.tx * V, mean, inv_std, gamma, beta);
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i)
+        if (i < mine) ch.template add<ACT>(xv[i], dv[i], s1, s2);
+    A* out1 = sums + at.image * g.channels + at.slab * g.width;
+    A* out2 = out1 + g.images * g.channels;
+    join_rows<THREADS, V>(g, 0, s1, s2, [&](int i, A t1, A t2) {
+        out1[i] = chan1[i] = t1;
+        out2[i] = chan2[i] = t2;
+    });
+    if (!dx) return;
+    __syncthreads();
+    for (int k = threadIdx.x / g.group_lanes; k < g.slab_groups; k += THREADS / g.group_lanes)
+        group_ab(chan1 + k * g.cg, chan2 + k * g.cg, gamma + at.slab * g.width + k * g.cg, 0, g.cg, 1, 0,
+                 (double)g.cg * g.pixels, g.group_lanes, &group_a[k], &group_b[k]);
+    __syncthreads();
+    if (!mine) return;
+    A a[V], b[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        a[j] = group_a[(at.tx * V + j) / g.cg];
+        b[j] = group_b[(at.tx * V + j) / g.cg];
+    }
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i)
+        if (i < mine) out[(at.ty + i * g.rows) * step] = ch.template apply<ACT>(xv[i], dv[i], a, b);
 }
 
 // ---------------------------------------------------------------------------------------------- channels first
@@ -402,7 +758,8 @@ __global__ void __launch_bounds__(kT) gn_first_apply(const T* __restrict__ x, co
     const long group = plane / cg;
     const int c = (int)(plane % channels);
     A mean, inv_std;
-    join_moments<A>(partial + group * cg, cg, [&](int) { return (double)pixels; }, (double)pixels * cg, eps, &mean, &inv_std);
+    join_moments<A>(partial + group * cg, cg, [&](int) { return (double)pixels; }, (double)pixels * cg, eps, kWave, &mean,
+                    &inv_std);
     if (plane % cg == 0 && threadIdx.x % THREADS == 0) {
         mean_out[group] = mean;
         inv_std_out[group] = inv_std;
@@ -468,61 +825,17 @@ __global__ void __launch_bounds__(kT) gn_first_bwd_apply(const T* __restrict__ d
     }
 }
 
-// ---------------------------------------------------------------------------------------------- joining the sums
-// A and B of each group from the channel sums of its runs: one wave a group.
+// A and B of each group: one wave a group.
 template <typename A>
 __global__ void __launch_bounds__(kT) gn_bwd_groups(const A* __restrict__ sums, const A* __restrict__ gamma,
-                                                    A* __restrict__ ab, long images, int splits, int channels, int groups,
-                                                    double m)
+                                                    A* __restrict__ ab, long images, int channels, int groups, double m)
 {
     const long group = (long)blockIdx.x * kWaves + threadIdx.x / kWave;
     if (group >= images * groups) return;
-    const int cg = channels / groups, c0 = (int)(group % groups) * cg;
-    const A* s1 = sums + (group / groups) * splits * channels;
-    const A* s2 = s1 + images * splits * channels;
-    double a = 0, b = 0;
-    for (int c = c0 + threadIdx.x % kWave; c < c0 + cg; c += kWave) {
-        double t1 = 0, t2 = 0;
-        for (int s = 0; s < splits; ++s) {
-            t1 += (double)s1[(long)s * channels + c];
-            t2 += (double)s2[(long)s * channels + c];
-        }
-        a += t1 * (double)gamma[c];
-        b += t2 * (double)gamma[c];
-    }
-    a = wave_sum(a);
-    b = wave_sum(b);
-    if (threadIdx.x % kWave == 0) {
-        ab[2 * group] = (A)(a / m);
-        ab[2 * group + 1] = (A)(b / m);
-    }
-}
-
-// dgamma and dbeta: the channel sums over images and runs.  A workgroup takes 16 channels, 16 threads each.
-template <typename A>
-__global__ void __launch_bounds__(kT) gn_bwd_params(const A* __restrict__ sums, A* __restrict__ dgamma,
-                                                    A* __restrict__ dbeta, long pieces, int channels)
-{
-    __shared__ double part1[kT], part2[kT];
-    const int c = blockIdx.x * 16 + threadIdx.x % 16, r = threadIdx.x / 16;
-    double t1 = 0, t2 = 0;
-    if (c < channels) {
-        for (long i = r; i < pieces; i += 16) {
-            t1 += (double)sums[i * channels + c];
-            t2 += (double)sums[(pieces + i) * channels + c];
-        }
-    }
-    part1[threadIdx.x] = t1;
-    part2[threadIdx.x] = t2;
-    __syncthreads();
-    if (r == 0 && c < channels) {
-        for (int k = 1; k < 16; ++k) {
-            t1 += part1[k * 16 + threadIdx.x];
-            t2 += part2[k * 16 + threadIdx.x];
-        }
-        dbeta[c] = (A)t1;
-        dgamma[c] = (A)t2;
-    }
+    const int cg = channels / groups;
+    const A* s1 = sums + (group / groups) * channels;
+    group_ab(s1, s1 + images * channels, gamma, (int)(group % groups) * cg, cg, 1, channels, m, kWave,
+             &ab[2 * group], &ab[2 * group + 1]);
 }
 
 // ---------------------------------------------------------------------------------------------- host
@@ -533,6 +846,22 @@ int pack_of(int size, int channels, int cg)
     int v = 16 / size;
     while (v > 1 && (channels % v || (channels / v > kT && cg % v))) v /= 2;
     return v;
+}
+
+// A power of two of the threads that `items` can have each, a wave at most.
+int lanes_of(int threads, int items)
+{
+    int lanes = kWave;
+    while (lanes > 1 && (long)lanes * items > threads) lanes /= 2;
+    return lanes;
+}
+
+void set_joins(GnLast* g, int threads, int v)
+{
+    const int unit = g->cg % v == 0 ? v : 1;
+    g->group_lanes = lanes_of(threads, g->slab_groups);
+    g->column_lanes = lanes_of(threads, g->tx * v);
+    g->by_columns = make_fastdiv((uint32_t)(g->slab_groups == 1 ? g->tx * (v / unit) : g->cg / unit));
 }
 
 GnLast last_shape(long images, int channels, int pixels, int groups, int v)
@@ -554,13 +883,39 @@ GnLast last_shape(long images, int channels, int pixels, int groups, int v)
     const int packs = g.width / v;
     g.tx = packs < kT ? packs : kT;
     g.rows = kT / g.tx;
-    // about eight workgroups to each of 256 compute units, and at least eight pixels to a thread
-    long want = (2048 + images * g.slabs - 1) / (images * g.slabs);
+    // three workgroups to each of 256 compute units, which hold them all at once (backward 64 x 56 x 56 x 256 in float32: 182 us
+    // against 188 with four and 199 with eight), and at least eight pixels to a thread
+    long want = (768 + images * g.slabs - 1) / (images * g.slabs);
     const long most = (pixels + 8l * g.rows - 1) / (8l * g.rows);
     if (want > most) want = most;
     g.run = (int)((pixels + want - 1) / want);
     g.splits = (pixels + g.run - 1) / g.run;
+    g.pieces = images * g.slabs * g.splits;
+    set_joins(&g, kT, v);
     return g;
+}
+
+// Where one kernel can hold a slab of an image in the registers of `threads` threads, `packs` packs of 16 bytes each (of x,
+// and in the backward pass as many of dy): the smallest slab of whole groups whose rows have at least `line` bytes, or all
+// channels.
+bool whole_shape(GnLast* g, long images, int channels, int pixels, int groups, int v, int size, int line, int threads,
+                 int packs)
+{
+    if (v * size != 16) return false;
+    const int cg = channels / groups;
+    for (int sg = 1; sg <= groups && (long)sg * cg <= kWholeWidth; ++sg) {
+        const int width = sg * cg;
+        if (groups % sg || width % v || (width * size < line && sg != groups)) continue;
+        const int tx = width / v;
+        // a slab of few packs leaves threads idle: it grows while there are workgroups enough
+        if (2l * pixels * tx < threads * packs && sg != groups && images * (groups / sg) > 1024) continue;
+        if (tx > threads || (pixels + threads / tx - 1) / (threads / tx) > packs) break;
+        *g = GnLast{images, pixels, channels, groups, cg, sg, width, groups / sg, tx, threads / tx, 1, pixels,
+                    images * (groups / sg), 1, 1, {}};
+        set_joins(g, threads, v);
+        return true;
+    }
+    return false;
 }
 
 int check(long images, long channels, long pixels, long groups)
@@ -625,6 +980,26 @@ bool too_many(long blocks) { return blocks * kT >= (1l << 32); }      // a launc
 // Planes of fewer pixels than this go to a wave each.
 constexpr int kPlaneOfGroup = 1024;
 
+// Calls launch(line, threads, packs) for the ways to hold a slab, the better first, until one fits: 256 threads before more
+// (several workgroups to a compute unit, whose loads and stores overlap) and whole lines of 128 bytes before half lines
+// (forward 64 x 14 x 14 x 1024 in float32: 19 us with lines, 22 with half lines).  The largest workgroup has a compute unit
+// to itself and is taken where one round of them does it all: forward 56 x 56 x 256 in float32 takes 22 us against 30 in two
+// passes for 16 images (256 slabs), 103 against 102 for 64.
+template <int FEW, int SOME_THREADS, int SOME, int MANY_THREADS, int MANY, typename F>
+bool hold_slabs(F launch)
+{
+    using std::integral_constant;
+    for (int line = 128; line >= 64; line /= 2)
+        if (launch(line, 1l << 40, integral_constant<int, 256>(), integral_constant<int, FEW>()) ||
+            launch(line, 1l << 40, integral_constant<int, SOME_THREADS>(), integral_constant<int, SOME>()))
+            return true;
+    for (int line = 128; line >= 64; line /= 2)
+        if (launch(line, 256l, integral_constant<int, MANY_THREADS>(), integral_constant<int, MANY>())) return true;
+    return false;
+}
+
+unsigned eights(long blocks) { return (unsigned)((blocks + 7) / 8 * 8); }
+
 template <typename T, int ACT>
 int forward(int nhwc, const T* x, const wide_t<T>* gamma, const wide_t<T>* beta, T* y, wide_t<T>* mean, wide_t<T>* inv_std,
             long images, int channels, int pixels, int groups, double eps, void* workspace, hipStream_t st)
@@ -633,13 +1008,28 @@ int forward(int nhwc, const T* x, const wide_t<T>* gamma, const wide_t<T>* beta,
     Moments<A>* part = static_cast<Moments<A>*>(workspace);
     if (nhwc) {
         const int v = aligned16(x) && aligned16(y) ? pack_of(sizeof(T), channels, channels / groups) : 1;
-        const GnLast g = last_shape(images, channels, pixels, groups, v);
-        const long blocks = images * g.slabs * g.splits;
-        if (too_many(blocks)) return PYDTNN_HIP_ERR_UNSUPPORTED;
+        GnLast g;
+        auto whole = [&](int line, long most, auto threads, auto packs) {
+            constexpr int N = decltype(threads)::value, M = decltype(packs)::value;
+            if (!whole_shape(&g, images, channels, pixels, groups, v, sizeof(T), line, N, M) || g.pieces > most ||
+                (g.pieces + 8) * N >= (1l << 32))
+                return false;
+            hipLaunchKernelGGL((gn_last_whole<T, 16 / (int)sizeof(T), ACT, N, M>), dim3(eights(g.pieces)), dim3(N), 0, st, x,
+                               gamma, beta, y, mean, inv_std, eps, g);
+            return true;
+        };
+        // packs of eight 16-bit values leave room for fewer threads
+        constexpr bool kShort = sizeof(T) == 2;
+        if (hold_slabs<4, 256, 16, kShort ? 512 : 1024, kShort ? 24 : 16>(whole)) {
+            HIP_RETURN_IF_LAUNCH_FAILED();
+            return PYDTNN_HIP_OK;
+        }
+        g = last_shape(images, channels, pixels, groups, v);
+        if (too_many(g.pieces + 8)) return PYDTNN_HIP_ERR_UNSUPPORTED;
         return with_pack(v, [&](auto pack) {
             constexpr int V = decltype(pack)::value * sizeof(T) <= 16 ? decltype(pack)::value : 1;
-            hipLaunchKernelGGL((gn_last_moments<T, V>), dim3((unsigned)blocks), dim3(kT), 0, st, x, part, g);
-            hipLaunchKernelGGL((gn_last_apply<T, V, ACT>), dim3((unsigned)blocks), dim3(kT), 0, st, x, gamma, beta, part, y,
+            hipLaunchKernelGGL((gn_last_moments<T, V>), dim3((unsigned)g.pieces), dim3(kT), 0, st, x, part, g);
+            hipLaunchKernelGGL((gn_last_apply<T, V, ACT>), dim3(eights(g.pieces)), dim3(kT), 0, st, x, gamma, beta, part, y,
                                mean, inv_std, eps, g);
             HIP_RETURN_IF_LAUNCH_FAILED();
             return PYDTNN_HIP_OK;
@@ -669,26 +1059,40 @@ int backward(int nhwc, const T* dy, const T* x, const wide_t<T>* gamma, const wi
     using A = wide_t<T>;
     A* sums = static_cast<A*>(workspace);
     const int cg = channels / groups;
-    const double m = (double)cg * pixels;
-    const unsigned group_blocks = (unsigned)((images * groups + kWaves - 1) / kWaves);
-    auto join = [&](long pieces, int splits) {
-        if (dx) hipLaunchKernelGGL((gn_bwd_groups<A>), dim3(group_blocks), dim3(kT), 0, st, sums, gamma, sums + 2 * pieces * channels,
-                                   images, splits, channels, groups, m);
-        hipLaunchKernelGGL((gn_bwd_params<A>), dim3((unsigned)((channels + 15) / 16)), dim3(kT), 0, st, sums, dgamma, dbeta,
-                           pieces, channels);
+    const int param_blocks = (channels + kParamChannels - 1) / kParamChannels;
+    auto params = [&](long pieces) {
+        hipLaunchKernelGGL((gn_bwd_params<A>), dim3((unsigned)param_blocks), dim3(kT), 0, st, sums, dgamma, dbeta, pieces,
+                           channels);
     };
     if (nhwc) {
         const int v = aligned16(x) && aligned16(dy) && aligned16(dx) ? pack_of(sizeof(T), channels, cg) : 1;
-        const GnLast g = last_shape(images, channels, pixels, groups, v);
-        const long blocks = images * g.slabs * g.splits;
-        if (too_many(blocks)) return PYDTNN_HIP_ERR_UNSUPPORTED;
+        GnLast g;
+        auto whole = [&](int line, long most, auto threads, auto packs) {
+            constexpr int N = decltype(threads)::value, M = decltype(packs)::value;
+            if (!whole_shape(&g, images, channels, pixels, groups, v, sizeof(T), line, N, M) || g.pieces > most ||
+                (g.pieces + 8) * N >= (1l << 32))
+                return false;
+            hipLaunchKernelGGL((gn_last_bwd_whole<T, 16 / (int)sizeof(T), ACT, N, M>), dim3(eights(g.pieces)), dim3(N), 0, st,
+                               dy, x, gamma, beta, mean, inv_std, sums, dx, g);
+            params(images);
+            return true;
+        };
+        constexpr bool kShort = sizeof(T) == 2;
+        if (hold_slabs<4, kShort ? 256 : 512, 8, kShort ? 512 : 1024, kShort ? 12 : 8>(whole)) {
+            HIP_RETURN_IF_LAUNCH_FAILED();
+            return PYDTNN_HIP_OK;
+        }
+        g = last_shape(images, channels, pixels, groups, v);
+        // the first workgroups of the second pass, in eights so that its pieces keep their dies, are those of the parameters
+        const long ahead = eights(param_blocks);
+        if (too_many(g.pieces + 8 + ahead)) return PYDTNN_HIP_ERR_UNSUPPORTED;
         return with_pack(v, [&](auto pack) {
             constexpr int V = decltype(pack)::value * sizeof(T) <= 16 ? decltype(pack)::value : 1;
-            hipLaunchKernelGGL((gn_last_bwd_sums<T, V, ACT>), dim3((unsigned)blocks), dim3(kT), 0, st, dy, x, gamma, beta,
+            hipLaunchKernelGGL((gn_last_bwd_sums<T, V, ACT>), dim3((unsigned)g.pieces), dim3(kT), 0, st, dy, x, gamma, beta,
                                mean, inv_std, sums, g);
-            join(images * g.splits, g.splits);
-            if (dx) hipLaunchKernelGGL((gn_last_bwd_apply<T, V, ACT>), dim3((unsigned)blocks), dim3(kT), 0, st, dy, x, gamma,
-                                       beta, mean, inv_std, sums + 2 * images * g.splits * channels, dx, g);
+            if (dx) hipLaunchKernelGGL((gn_last_bwd_apply<T, V, ACT>), dim3((unsigned)(ahead + eights(g.pieces))), dim3(kT), 0,
+                                       st, dy, x, gamma, beta, mean, inv_std, sums, dgamma, dbeta, dx, (int)ahead, g);
+            else params(images * g.splits);
             HIP_RETURN_IF_LAUNCH_FAILED();
             return PYDTNN_HIP_OK;
         });
@@ -699,11 +1103,15 @@ int backward(int nhwc, const T* dy, const T* x, const wide_t<T>* gamma, const wi
     if (too_many(blocks)) return PYDTNN_HIP_ERR_UNSUPPORTED;
     auto launch = [&](auto threads) {
         constexpr int N = decltype(threads)::value;
+        A* ab = sums + 2 * planes;
         hipLaunchKernelGGL((gn_first_bwd_sums<T, N, ACT>), dim3((unsigned)blocks), dim3(kT), 0, st, dy, x, gamma, beta, mean,
                            inv_std, sums, planes, pixels, channels, cg);
-        join(images, 1);
-        if (dx) hipLaunchKernelGGL((gn_first_bwd_apply<T, N, ACT>), dim3((unsigned)blocks), dim3(kT), 0, st, dy, x, gamma, beta,
-                                   mean, inv_std, sums + 2 * planes, dx, planes, pixels, channels, cg);
+        params(images);
+        if (!dx) return;
+        hipLaunchKernelGGL((gn_bwd_groups<A>), dim3((unsigned)((images * groups + kWaves - 1) / kWaves)), dim3(kT), 0, st, sums,
+                           gamma, ab, images, channels, groups, (double)cg * pixels);
+        hipLaunchKernelGGL((gn_first_bwd_apply<T, N, ACT>), dim3((unsigned)blocks), dim3(kT), 0, st, dy, x, gamma, beta, mean,
+                           inv_std, ab, dx, planes, pixels, channels, cg);
     };
     if (small) launch(std::integral_constant<int, kWave>());
     else launch(std::integral_constant<int, kT>());

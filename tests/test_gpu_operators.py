@@ -59,6 +59,12 @@ GN_SHAPES = [
     (2, (65, 63), 8, 2),           # many pixels: runs
     (1, (40, 41), 320, 32),        # runs of an image with idle threads
     (1500, (2, 2), 4, 2),          # many small images
+    (2, (28, 28), 64, 8),          # slabs that a workgroup's registers hold: of several sizes of workgroup
+    (1, (27, 29), 48, 1),
+    (3, (14, 13), 160, 10),
+    (1, (56, 55), 32, 4),
+    (1, (56, 57), 96, 6),
+    (2, (90, 80), 32, 16),         # and slabs that they do not
 ]
 
 
