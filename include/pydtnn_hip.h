@@ -484,9 +484,10 @@ int pydtnn_hip_dropout(int dtype, const void *x, void *y, long total, double rat
  *       the way and wq (n, kp), wscales as pydtnn_hip_quantize_fp8 makes them of the (n, k) weights, once.  bias (n) is
  *       float32 or NULL; sums are held in float32.
  * x and y are float32, float16 or bfloat16 (`dtype`; PYDTNN_HIP_ERR_INVALID for float64).  q and the workspace are aligned to
- * 16 bytes, scales to 4.  Extents are at most 2^30.  Workspace: pydtnn_hip_matmul_fp8_workspace_bytes(m, n, k). */
+ * 16 bytes, scales to 4.  m and n are at most 2^30, k at most 2^23.  Workspace:
+ * pydtnn_hip_matmul_fp8_workspace_bytes(dtype, m, n, k). */
 int pydtnn_hip_quantize_fp8(int dtype, const void *x, long rows, long k, uint8_t *q, uint8_t *scales, void *stream);
-size_t pydtnn_hip_matmul_fp8_workspace_bytes(long m, long n, long k);
+size_t pydtnn_hip_matmul_fp8_workspace_bytes(int dtype, long m, long n, long k);
 int pydtnn_hip_matmul_fp8(int dtype, const void *x, long m, long k, const uint8_t *wq, const uint8_t *wscales, long n,
                           const float *bias, int relu, void *y, void *workspace, size_t workspace_bytes, void *stream);
 

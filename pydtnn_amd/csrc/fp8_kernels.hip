@@ -117,37 +117,272 @@ __device__ __forceinline__ v4f block_product(v8i w, int we, v8i x, int xe, v4f a
     return acc;
 }
 
-// One wave computes 16 n by 16 m.  The weights are the first operand, so that a lane ends with four consecutive n of one m.
+// bias, ReLU and the one rounding to the type of the result
 template <typename T>
-__global__ void __launch_bounds__(kT) matmul_fp8_kernel(const uint8_t* __restrict__ xq, const uint32_t* __restrict__ xs,
-                                                        const uint8_t* __restrict__ wq, const uint32_t* __restrict__ ws,
-                                                        const float* __restrict__ bias, T* __restrict__ y, Fp8Shape s,
-                                                        int relu)
+__device__ __forceinline__ T finish(float v, const float* bias, long n, int relu)
 {
-    const int lane = threadIdx.x % kWave, row = lane % 16, part = lane / 16;
-    const long n0 = (long)blockIdx.x * 64 + threadIdx.x / kWave * 16, m0 = (long)blockIdx.y * 16;
-    const long wr = min(n0 + row, s.n - 1), xr = min(m0 + row, s.m - 1);
-    const long kp = (long)s.blocks * kBlock;
-    const v4i* wp = reinterpret_cast<const v4i*>(wq + wr * kp + part * 32);
-    const v4i* xp = reinterpret_cast<const v4i*>(xq + xr * kp + part * 32);
-    v4f acc = {0, 0, 0, 0};
-    for (int b = 0; b < s.blocks; ++b) {
-        const v4i w0 = wp[b * 8], w1 = wp[b * 8 + 1], x0 = xp[b * 8], x1 = xp[b * 8 + 1];
-        const v8i wv = {w0[0], w0[1], w0[2], w0[3], w1[0], w1[1], w1[2], w1[3]};
-        const v8i xv = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
-        const int we = (int)(ws[wr * s.words + b / 4] >> (b % 4 * 8)), xe = (int)(xs[xr * s.words + b / 4] >> (b % 4 * 8));
-        acc = block_product<sizeof(T) == 4>(wv, we, xv, xe, acc);
-    }
-    const long m = m0 + row;
-    if (m >= s.m) return;
+    if (bias) v += bias[n];
+    if (relu) v = v > 0.0f ? v : 0.0f;
+    return (T)v;
+}
+
+// Four consecutive n of one m.
+template <typename T>
+__device__ __forceinline__ void store_four(T* y, long m, long n, const Fp8Shape& s, v4f v, const float* bias, int relu)
+{
+    T* to = y + m * s.n + n;
+    if (n + 4 <= s.n && s.n % 4 == 0 && ((uintptr_t)y & (4 * sizeof(T) - 1)) == 0) {
+        Pack<T, 4> out;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const long n = n0 + part * 4 + i;
-        if (n >= s.n) return;
-        float v = acc[i] + (bias ? bias[n] : 0.0f);
-        if (relu) v = v > 0.0f ? v : 0.0f;
-        y[m * s.n + n] = (T)v;
+        for (int i = 0; i < 4; ++i) out.v[i] = finish<T>(v[i], bias, n + i, relu);
+        *reinterpret_cast<Pack<T, 4>*>(to) = out;
+        return;
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (n + i < s.n) to[i] = finish<T>(v[i], bias, n + i, relu);
+}
+
+// ---------------------------------------------------------------------------------------------- few rows
+// Up to 16 * MT rows of x: bound by reading the weights, each of which is used for those rows only.  A workgroup takes 16
+// rows of the weights; its waves take the words of four blocks in turn, with the next word's operands on their way while
+// the present one's are multiplied, and join their sums in local memory, in the order of the waves.  The weights are the
+// first operand, so that a lane ends with four consecutive n of one m.
+constexpr int kFewWaves = 8;
+
+template <int MT>
+struct WordOfBlocks {
+    v4i w[4][2], x[MT][4][2];
+    int we, xe[MT];
+
+    __device__ __forceinline__ void load(const v4i* wp, const v4i* const (&xp)[MT], const uint32_t* wsp,
+                                         const uint32_t* const (&xsp)[MT], int word, int blocks)
+    {
+        we = (int)wsp[word];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) xe[t] = (int)xsp[t][word];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const long at = (long)min(word * 4 + b, blocks - 1) * (kBlock / 16);
+            w[b][0] = wp[at], w[b][1] = wp[at + 4];
+#pragma unroll
+            for (int t = 0; t < MT; ++t) x[t][b][0] = xp[t][at], x[t][b][1] = xp[t][at + 4];
+        }
+    }
+};
+
+__device__ __forceinline__ v8i join(v4i a, v4i b)
+{
+    return v8i{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+
+template <typename T, int MT>
+__global__ void __launch_bounds__(kFewWaves* kWave) matmul_fp8_few_kernel(const uint8_t* __restrict__ xq,
+                                                                          const uint32_t* __restrict__ xs,
+                                                                          const uint8_t* __restrict__ wq,
+                                                                          const uint32_t* __restrict__ ws,
+                                                                          const float* __restrict__ bias, T* __restrict__ y,
+                                                                          Fp8Shape s, int relu)
+{
+    constexpr bool EXACT = sizeof(T) == 4;
+    __shared__ v4f part[kFewWaves][MT][kWave];
+    const int lane = threadIdx.x % kWave, row = lane % 16, piece = lane / 16, wave = threadIdx.x / kWave;
+    const long n0 = (long)blockIdx.x * 16;
+    const long wr = min(n0 + row, s.n - 1), kp = (long)s.blocks * kBlock;
+    const v4i* wp = reinterpret_cast<const v4i*>(wq + wr * kp) + piece;
+    const uint32_t* wsp = ws + wr * s.words;
+    const v4i* xp[MT];
+    const uint32_t* xsp[MT];
+    v4f acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const long xr = min((long)t * 16 + row, s.m - 1);
+        xp[t] = reinterpret_cast<const v4i*>(xq + xr * kp) + piece;
+        xsp[t] = xs + xr * s.words;
+        acc[t] = v4f{0, 0, 0, 0};
+    }
+    WordOfBlocks<MT> now, next;
+    if (wave < s.words) now.load(wp, xp, wsp, xsp, wave, s.blocks);
+    for (int word = wave; word < s.words; word += kFewWaves) {
+        next.load(wp, xp, wsp, xsp, min(word + kFewWaves, s.words - 1), s.blocks);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            if (word * 4 + b >= s.blocks) break;
+            const v8i w = join(now.w[b][0], now.w[b][1]);
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+                acc[t] = block_product<EXACT>(w, now.we >> (8 * b), join(now.x[t][b][0], now.x[t][b][1]), now.xe[t] >> (8 * b),
+                                              acc[t]);
+        }
+        now = next;
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) part[wave][t][lane] = acc[t];
+    __syncthreads();
+    for (int t = wave; t < MT; t += kFewWaves) {
+        v4f sum = part[0][t][lane];
+#pragma unroll
+        for (int v = 1; v < kFewWaves; ++v) sum += part[v][t][lane];
+        if (t * 16 + row < s.m && n0 + piece * 4 < s.n) store_four(y, (long)t * 16 + row, n0 + piece * 4, s, sum, bias, relu);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- tiles
+// A workgroup of WN x WM waves computes BN rows of the weights by BM rows of x.  A step is one block of 128 k: its BN + BM
+// rows of 128 bytes go to local memory by loads that write there directly, STAGES - 1 steps ahead of their use.  The
+// eight 16-byte pieces of a row r stand at place piece ^ (r % 8), so that the sixteen rows that a fragment reads at once fall
+// on different banks; the loads' lanes pick their pieces accordingly, and since a lane's two pieces of a block are any two,
+// as long as both operands take the same, a lane takes pieces p and p + 4.
+typedef __attribute__((address_space(3))) void LdsVoid;
+
+typedef __amdgpu_buffer_rsrc_t Rows;
+
+// Rows from `base`; those behind the last byte read as zeros.
+__device__ __forceinline__ Rows rows_of(const uint8_t* base, long bytes)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, (int)(uint32_t)min(bytes, 0xffffffffl), 0x00020000);
+}
+
+template <int N>
+__device__ __forceinline__ void wait_loads()
+{
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+template <typename T, bool EXACT, int BN, int BM, int WN, int WM, int STAGES>
+__global__ void __launch_bounds__(WN* WM* kWave, STAGES * (BN + BM) * kBlock > 80 * 1024 ? 1 : 2)
+    matmul_fp8_tile_kernel(const uint8_t* __restrict__ xq, const uint32_t* __restrict__ xs, const uint8_t* __restrict__ wq,
+                           const uint32_t* __restrict__ ws, const float* __restrict__ bias, T* __restrict__ y,
+                           float* __restrict__ partial, Fp8Shape s, int relu, int tiles_n, int tiles_m, int splits)
+{
+    constexpr int WAVES = WN * WM, TN = BN / WN / 16, TM = BM / WM / 16;
+    constexpr int WLOADS = BN / 8 / WAVES, LOADS = (BN + BM) / 8 / WAVES;     // loads of a wave and step: eight rows each
+    constexpr int STAGE = (BN + BM) * kBlock;
+    __shared__ __attribute__((aligned(128))) uint8_t lds[STAGES * STAGE];
+
+    // Consecutive workgroups go to the eight dies in turn; a die's tiles are consecutive, in bands of four tiles of n, so that
+    // its second-level cache holds what they share.
+    const long tiles = (long)tiles_n * tiles_m * splits, share = (tiles + 7) / 8;
+    const long place = (long)(blockIdx.x % 8) * share + blockIdx.x / 8;
+    if (blockIdx.x / 8 >= share || place >= tiles) return;
+    const int split = (int)(place % splits);
+    const long tile = place / splits;
+    const int band = (int)(tile / (4l * tiles_m)), in_band = (int)(tile % (4l * tiles_m));
+    const int band_n = min(4, tiles_n - band * 4);
+    const long n0 = (band * 4l + in_band % band_n) * BN, m0 = (long)(in_band / band_n) * BM;
+
+    const int words = (s.words + splits - 1) / splits;      // of a split
+    const int first = split * words * 4, last = min((split + 1) * words * 4, s.blocks);
+
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int row = lane % 16, piece = lane / 16, wn = wave % WN, wm = wave / WN;
+    const long kp = (long)s.blocks * kBlock;
+    const Rows wres = rows_of(wq + n0 * kp, (s.n - n0) * kp), xres = rows_of(xq + m0 * kp, (s.m - m0) * kp);
+    uint32_t from[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const int r = (wave + (i < WLOADS ? i : i - WLOADS) * WAVES) * 8 + lane / 8;
+        from[i] = (uint32_t)(r * kp) + (uint32_t)(((lane % 8) ^ (lane / 8)) * 16);
+    }
+    auto issue = [&](int step, int stage) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int group = i < WLOADS ? wave + i * WAVES : BN / 8 + wave + (i - WLOADS) * WAVES;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(i < WLOADS ? wres : xres, (LdsVoid*)(lds + stage * STAGE + group * 1024), 16,
+                                                     (int)from[i], step * kBlock, 0, 0);
+        }
+    };
+
+    const uint32_t* wsp[TN];
+    const uint32_t* xsp[TM];
+#pragma unroll
+    for (int i = 0; i < TN; ++i) wsp[i] = ws + min(n0 + wn * TN * 16 + i * 16 + row, s.n - 1) * s.words;
+#pragma unroll
+    for (int j = 0; j < TM; ++j) xsp[j] = xs + min(m0 + wm * TM * 16 + j * 16 + row, s.m - 1) * s.words;
+    int we[TN], xe[TM], we_next[TN], xe_next[TM];
+    auto scales = [&](int word) {
+#pragma unroll
+        for (int i = 0; i < TN; ++i) we_next[i] = (int)wsp[i][word];
+#pragma unroll
+        for (int j = 0; j < TM; ++j) xe_next[j] = (int)xsp[j][word];
+    };
+
+    v4f acc[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j) acc[i][j] = v4f{0, 0, 0, 0};
+
+    if (first < last) {
+        scales(first / 4);
+#pragma unroll
+        for (int t = 0; t < STAGES - 1; ++t)
+            if (first + t < last) issue(first + t, t);
+    }
+    const uint32_t mine = (uint32_t)((row * kBlock) + ((piece ^ (row % 8)) * 16));
+    const uint32_t wbase = (uint32_t)(wn * TN * 16 * kBlock) + mine, xbase = (uint32_t)((BN + wm * TM * 16) * kBlock) + mine;
+    int stage = 0;
+    for (int step = first; step < last; ++step) {
+        if (step % 4 == 0) {
+#pragma unroll
+            for (int i = 0; i < TN; ++i) we[i] = we_next[i];
+#pragma unroll
+            for (int j = 0; j < TM; ++j) xe[j] = xe_next[j];
+            scales(min(step / 4 + 1, s.words - 1));
+        } else {
+#pragma unroll
+            for (int i = 0; i < TN; ++i) we[i] = (int)((uint32_t)we[i] >> 8);
+#pragma unroll
+            for (int j = 0; j < TM; ++j) xe[j] = (int)((uint32_t)xe[j] >> 8);
+        }
+        // this step's loads are the oldest; while later steps' follow them, those may stay under way
+        if (STAGES > 2 && step + STAGES - 2 < last) wait_loads<(STAGES - 2) * LOADS>();
+        else wait_loads<0>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");      // no access moves across the barrier
+        if (step + STAGES - 1 < last) issue(step + STAGES - 1, (stage + STAGES - 1) % STAGES);
+        const uint8_t* here = lds + stage * STAGE;
+        v8i x[TM];
+#pragma unroll
+        for (int j = 0; j < TM; ++j)
+            x[j] = join(*reinterpret_cast<const v4i*>(here + xbase + j * 16 * kBlock),
+                        *reinterpret_cast<const v4i*>(here + (xbase ^ 64u) + j * 16 * kBlock));
+#pragma unroll
+        for (int i = 0; i < TN; ++i) {
+            const v8i w = join(*reinterpret_cast<const v4i*>(here + wbase + i * 16 * kBlock),
+                               *reinterpret_cast<const v4i*>(here + (wbase ^ 64u) + i * 16 * kBlock));
+#pragma unroll
+            for (int j = 0; j < TM; ++j) acc[i][j] = block_product<EXACT>(w, we[i], x[j], xe[j], acc[i][j]);
+        }
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+    }
+
+#pragma unroll
+    for (int i = 0; i < TN; ++i) {
+        const long n = n0 + wn * TN * 16 + i * 16 + piece * 4;
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+            const long m = m0 + wm * TM * 16 + j * 16 + row;
+            if (m >= s.m || n >= s.n) continue;
+            if (splits == 1) {
+                store_four(y, m, n, s, acc[i][j], bias, relu);
+            } else {
+                store_four(partial + split * s.m * s.n, m, n, s, acc[i][j], nullptr, 0);
+            }
+        }
+    }
+}
+
+// The sum of the splits' results, in order.
+template <typename T>
+__global__ void __launch_bounds__(kT) join_splits_kernel(const float* __restrict__ partial, const float* __restrict__ bias,
+                                                         T* __restrict__ y, long m, long n, int splits, int relu)
+{
+    const long i = (long)blockIdx.x * kT + threadIdx.x;
+    if (i >= m * n) return;
+    float v = partial[i];
+    for (int k = 1; k < splits; ++k) v += partial[k * m * n + i];
+    y[i] = finish<T>(v, bias, i % n, relu);
 }
 
 bool shape_of(Fp8Shape* s, long m, long n, long k)
@@ -158,6 +393,39 @@ bool shape_of(Fp8Shape* s, long m, long n, long k)
 }
 
 size_t q_bytes(const Fp8Shape& s) { return (size_t)s.m * s.blocks * kBlock; }
+size_t scale_bytes(const Fp8Shape& s) { return ((size_t)s.m * s.words * 4 + 15) / 16 * 16; }
+
+constexpr long kFewRows = 32;
+constexpr int kSplitsMost = 16;
+
+// Tiles of `size` by `size`, and how many pieces k is cut into: where there are fewer tiles than 256 compute units, until
+// there are about twice as many, each with at least four words of four blocks.
+struct Tiling {
+    int size, splits;
+};
+
+Tiling tiling_of(const Fp8Shape& s, bool exact)
+{
+    auto tiles = [&](long size) { return ((s.m + size - 1) / size) * ((s.n + size - 1) / size); };
+    Tiling t = {64, 1};
+    if (!exact && tiles(256) >= 192) t.size = 256;
+    else if (tiles(128) >= 192) t.size = 128;
+    const long count = tiles(t.size);
+    if (count < 256) {
+        long splits = 512 / count;
+        if (splits > s.words / 2) splits = s.words / 2;
+        if (splits > kSplitsMost) splits = kSplitsMost;
+        if (splits > 1) t.splits = (int)splits;
+    }
+    return t;
+}
+
+size_t partial_bytes(const Fp8Shape& s, bool exact)
+{
+    if (s.m <= kFewRows) return 0;
+    const Tiling t = tiling_of(s, exact);
+    return t.splits > 1 ? (size_t)t.splits * s.m * s.n * 4 : 0;
+}
 
 template <typename F>
 int with_fp8_input(int dtype, F f)
@@ -187,7 +455,54 @@ int quantize(const T* x, long rows, long k, uint8_t* q, uint8_t* scales, hipStre
     return PYDTNN_HIP_OK;
 }
 
-constexpr long kMost = 1l << 30;      // rows and columns are counted in 32 bits
+template <typename T, bool EXACT, int BN, int BM, int WN, int WM, int STAGES>
+int launch_tiles(const uint8_t* xq, const uint8_t* xs, const uint8_t* wq, const uint8_t* ws, const float* bias, T* y,
+                 float* partial, const Fp8Shape& s, int relu, int splits, hipStream_t st)
+{
+    const long tiles_n = (s.n + BN - 1) / BN, tiles_m = (s.m + BM - 1) / BM;
+    const long blocks = (tiles_n * tiles_m * splits + 7) / 8 * 8;
+    if (blocks * WN * WM * kWave >= (1l << 32)) return PYDTNN_HIP_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((matmul_fp8_tile_kernel<T, EXACT, BN, BM, WN, WM, STAGES>), dim3((unsigned)blocks), dim3(WN * WM * kWave),
+                       0, st, xq, (const uint32_t*)xs, wq, (const uint32_t*)ws, bias, y, partial, s, relu, (int)tiles_n,
+                       (int)tiles_m, splits);
+    HIP_RETURN_IF_LAUNCH_FAILED();
+    if (splits == 1) return PYDTNN_HIP_OK;
+    const long join = (s.m * s.n + kT - 1) / kT;
+    if (join * kT >= (1l << 32)) return PYDTNN_HIP_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((join_splits_kernel<T>), dim3((unsigned)join), dim3(kT), 0, st, partial, bias, y, s.m, s.n, splits, relu);
+    HIP_RETURN_IF_LAUNCH_FAILED();
+    return PYDTNN_HIP_OK;
+}
+
+template <typename T>
+int product(const uint8_t* xq, const uint8_t* xs, const uint8_t* wq, const uint8_t* ws, const float* bias, T* y, float* partial,
+            const Fp8Shape& s, int relu, hipStream_t st)
+{
+    constexpr bool EXACT = sizeof(T) == 4;
+    if (s.m <= kFewRows) {
+        const long blocks = (s.n + 15) / 16;
+        if (blocks * kFewWaves * kWave >= (1l << 32)) return PYDTNN_HIP_ERR_UNSUPPORTED;
+        auto few = [&](auto tiles) {
+            hipLaunchKernelGGL((matmul_fp8_few_kernel<T, decltype(tiles)::value>), dim3((unsigned)blocks),
+                               dim3(kFewWaves * kWave), 0, st, xq, (const uint32_t*)xs, wq, (const uint32_t*)ws, bias, y, s,
+                               relu);
+        };
+        if (s.m <= 16) few(std::integral_constant<int, 1>());
+        else few(std::integral_constant<int, 2>());
+        HIP_RETURN_IF_LAUNCH_FAILED();
+        return PYDTNN_HIP_OK;
+    }
+    const Tiling t = tiling_of(s, EXACT);
+    if constexpr (!EXACT)
+        if (t.size == 256)
+            return launch_tiles<T, EXACT, 256, 256, 2, 4, 2>(xq, xs, wq, ws, bias, y, partial, s, relu, t.splits, st);
+    if (t.size == 128) return launch_tiles<T, EXACT, 128, 128, 2, 2, 2>(xq, xs, wq, ws, bias, y, partial, s, relu, t.splits, st);
+    return launch_tiles<T, EXACT, 64, 64, 2, 2, 4>(xq, xs, wq, ws, bias, y, partial, s, relu, t.splits, st);
+}
+
+constexpr long kMost = 1l << 30, kMostK = 1l << 23;      // rows are counted, and a tile's rows addressed, in 32 bits
+
+bool too_large(long m, long n, long k) { return m > kMost || n > kMost || k > kMostK; }
 
 }  // namespace
 
@@ -197,18 +512,18 @@ int pydtnn_hip_quantize_fp8(int dtype, const void* x, long rows, long k, uint8_t
 {
     if (!x || !q || !scales) return PYDTNN_HIP_ERR_INVALID;
     if (!aligned16(q) || ((uintptr_t)scales & 3)) return PYDTNN_HIP_ERR_INVALID;
-    if (rows > kMost || k > kMost) return PYDTNN_HIP_ERR_UNSUPPORTED;
+    if (too_large(rows, 1, k)) return PYDTNN_HIP_ERR_UNSUPPORTED;
     return with_fp8_input(dtype, [&](auto t) {
         using T = decltype(t);
         return quantize<T>((const T*)x, rows, k, q, scales, convint::as_stream(stream));
     });
 }
 
-size_t pydtnn_hip_matmul_fp8_workspace_bytes(long m, long n, long k)
+size_t pydtnn_hip_matmul_fp8_workspace_bytes(int dtype, long m, long n, long k)
 {
     Fp8Shape s;
-    if (!shape_of(&s, m, n, k) || m > kMost || n > kMost || k > kMost) return 0;
-    return q_bytes(s) + (size_t)m * s.words * 4;
+    if (!shape_of(&s, m, n, k) || too_large(m, n, k)) return 0;
+    return q_bytes(s) + scale_bytes(s) + partial_bytes(s, dtype == kDtypeF32);
 }
 
 int pydtnn_hip_matmul_fp8(int dtype, const void* x, long m, long k, const uint8_t* wq, const uint8_t* wscales, long n,
@@ -217,20 +532,19 @@ int pydtnn_hip_matmul_fp8(int dtype, const void* x, long m, long k, const uint8_
     Fp8Shape s;
     if (!x || !wq || !wscales || !y || !shape_of(&s, m, n, k)) return PYDTNN_HIP_ERR_INVALID;
     if (!aligned16(wq) || ((uintptr_t)wscales & 3)) return PYDTNN_HIP_ERR_INVALID;
-    if (m > kMost || n > kMost || k > kMost || (m + 15) / 16 > 65535) return PYDTNN_HIP_ERR_UNSUPPORTED;
-    if (!workspace || !aligned16(workspace) || workspace_bytes < pydtnn_hip_matmul_fp8_workspace_bytes(m, n, k))
+    if (too_large(m, n, k)) return PYDTNN_HIP_ERR_UNSUPPORTED;
+    if (dtype == kDtypeF64) return PYDTNN_HIP_ERR_INVALID;
+    if (!workspace || !aligned16(workspace) || workspace_bytes < pydtnn_hip_matmul_fp8_workspace_bytes(dtype, m, n, k))
         return PYDTNN_HIP_ERR_WORKSPACE;
     return with_fp8_input(dtype, [&](auto t) {
         using T = decltype(t);
         const hipStream_t st = convint::as_stream(stream);
         uint8_t* xq = static_cast<uint8_t*>(workspace);
         uint8_t* xs = xq + q_bytes(s);
+        float* partial = reinterpret_cast<float*>(xs + scale_bytes(s));
         const int rc = quantize<T>((const T*)x, m, k, xq, xs, st);
         if (rc != PYDTNN_HIP_OK) return rc;
-        hipLaunchKernelGGL((matmul_fp8_kernel<T>), dim3((unsigned)((n + 63) / 64), (unsigned)((m + 15) / 16)), dim3(kT), 0, st,
-                           xq, (const uint32_t*)xs, wq, (const uint32_t*)wscales, bias, (T*)y, s, relu);
-        HIP_RETURN_IF_LAUNCH_FAILED();
-        return PYDTNN_HIP_OK;
+        return product<T>(xq, xs, wq, wscales, bias, (T*)y, partial, s, relu, st);
     });
 }
 

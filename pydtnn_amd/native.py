@@ -119,7 +119,7 @@ SIGNATURES = {
                                                                                           _vp]),
     "pydtnn_hip_dropout": (_c.c_int, [_c.c_int, _vp, _vp, _c.c_long, _c.c_double, _c.c_uint64, _c.c_uint64, _vp, _vp]),
     "pydtnn_hip_quantize_fp8": (_c.c_int, [_c.c_int, _vp, _c.c_long, _c.c_long, _vp, _vp, _vp]),
-    "pydtnn_hip_matmul_fp8_workspace_bytes": (_c.c_size_t, [_c.c_long] * 3),
+    "pydtnn_hip_matmul_fp8_workspace_bytes": (_c.c_size_t, [_c.c_int] + [_c.c_long] * 3),
     "pydtnn_hip_matmul_fp8": (_c.c_int, [_c.c_int, _vp, _c.c_long, _c.c_long, _vp, _vp, _c.c_long, _vp, _c.c_int, _vp, _vp,
                                          _c.c_size_t, _vp]),
 }

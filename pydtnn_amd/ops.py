@@ -699,7 +699,7 @@ def matmul_fp8(x, wq, wscales, bias=None, relu=False):
     x = x.contiguous()
     y = torch.empty((m, n), dtype=x.dtype, device=x.device)
     if m:
-        nbytes = lib().pydtnn_hip_matmul_fp8_workspace_bytes(m, n, k)
+        nbytes = lib().pydtnn_hip_matmul_fp8_workspace_bytes(dtype, m, n, k)
         ws = _scratch(nbytes, x)
         check(lib().pydtnn_hip_matmul_fp8(dtype, ptr(x), m, k, ptr(wq), ptr(wscales), n, ptr(bias), int(relu), ptr(y), ptr(ws),
                                           nbytes, stream_ptr()), "matmul_fp8")

@@ -165,7 +165,7 @@ def test_fp8_refuses_what_it_cannot_run(lib):
     assert quantize(k=(1 << 30) + 1) == 4
 
     def matmul(dtype=0, m=4, k=200, n=6, x=p, w=p, s=p, y=p, ws=p, short=0):
-        need = lib.pydtnn_hip_matmul_fp8_workspace_bytes(m, n, k)
+        need = lib.pydtnn_hip_matmul_fp8_workspace_bytes(dtype, m, n, k)
         return lib.pydtnn_hip_matmul_fp8(dtype, x, m, k, w, s, n, None, 0, y, ws, max(need - short, 0), None)
 
     assert matmul(x=None) == matmul(w=None) == matmul(s=None) == matmul(y=None) == 1
