@@ -150,6 +150,11 @@ __device__ __forceinline__ void store_four(T* y, long m, long n, const Fp8Shape&
 // first operand, so that a lane ends with four consecutive n of one m.
 constexpr int kFewWaves = 8;
 
+__device__ __forceinline__ v8i join(v4i a, v4i b)
+{
+    return v8i{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+
 template <int MT>
 struct WordOfBlocks {
     v4i w[4][2], x[MT][4][2];
@@ -169,12 +174,20 @@ struct WordOfBlocks {
             for (int t = 0; t < MT; ++t) x[t][b][0] = xp[t][at], x[t][b][1] = xp[t][at + 4];
         }
     }
-};
 
-__device__ __forceinline__ v8i join(v4i a, v4i b)
-{
-    return v8i{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-}
+    template <bool EXACT>
+    __device__ __forceinline__ void multiply(int word, int blocks, v4f (&acc)[MT]) const
+    {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            if (word * 4 + b >= blocks) break;
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+                acc[t] = block_product<EXACT>(join(w[b][0], w[b][1]), we >> (8 * b), join(x[t][b][0], x[t][b][1]),
+                                              xe[t] >> (8 * b), acc[t]);
+        }
+    }
+};
 
 template <typename T, int MT>
 __global__ void __launch_bounds__(kFewWaves* kWave) matmul_fp8_few_kernel(const uint8_t* __restrict__ xq,
@@ -201,20 +214,15 @@ __global__ void __launch_bounds__(kFewWaves* kWave) matmul_fp8_few_kernel(const 
         xsp[t] = xs + xr * s.words;
         acc[t] = v4f{0, 0, 0, 0};
     }
-    WordOfBlocks<MT> now, next;
-    if (wave < s.words) now.load(wp, xp, wsp, xsp, wave, s.blocks);
-    for (int word = wave; word < s.words; word += kFewWaves) {
-        next.load(wp, xp, wsp, xsp, min(word + kFewWaves, s.words - 1), s.blocks);
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            if (word * 4 + b >= s.blocks) break;
-            const v8i w = join(now.w[b][0], now.w[b][1]);
-#pragma unroll
-            for (int t = 0; t < MT; ++t)
-                acc[t] = block_product<EXACT>(w, now.we >> (8 * b), join(now.x[t][b][0], now.x[t][b][1]), now.xe[t] >> (8 * b),
-                                              acc[t]);
-        }
-        now = next;
+    // two words in turn, without a copy from one to the other: a copy would wait for the loads
+    WordOfBlocks<MT> even, odd;
+    if (wave < s.words) even.load(wp, xp, wsp, xsp, wave, s.blocks);
+    for (int word = wave; word < s.words; word += 2 * kFewWaves) {
+        odd.load(wp, xp, wsp, xsp, min(word + kFewWaves, s.words - 1), s.blocks);
+        even.template multiply<EXACT>(word, s.blocks, acc);
+        if (word + kFewWaves >= s.words) break;
+        even.load(wp, xp, wsp, xsp, min(word + 2 * kFewWaves, s.words - 1), s.blocks);
+        odd.template multiply<EXACT>(word + kFewWaves, s.blocks, acc);
     }
 #pragma unroll
     for (int t = 0; t < MT; ++t) part[wave][t][lane] = acc[t];
@@ -233,20 +241,94 @@ __global__ void __launch_bounds__(kFewWaves* kWave) matmul_fp8_few_kernel(const 
 // eight 16-byte pieces of a row r stand at place piece ^ (r % 8), so that the sixteen rows that a fragment reads at once fall
 // on different banks; the loads' lanes pick their pieces accordingly, and since a lane's two pieces of a block are any two,
 // as long as both operands take the same, a lane takes pieces p and p + 4.
-typedef __attribute__((address_space(3))) void LdsVoid;
-
-typedef __amdgpu_buffer_rsrc_t Rows;
+typedef v4i Rows;      // a buffer resource
 
 // Rows from `base`; those behind the last byte read as zeros.
-__device__ __forceinline__ Rows rows_of(const uint8_t* base, long bytes)
+__device__ __forceinline__ Rows rows_of(const void* base, long bytes)
 {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, (int)(uint32_t)min(bytes, 0xffffffffl), 0x00020000);
+    return Rows{(int)(uint32_t)(uintptr_t)base, (int)((uintptr_t)base >> 32), (int)(uint32_t)min(bytes, 0xffffffffl), 0x00020000};
+}
+
+// m0 is set here and nowhere else; the compiler warns that it reserves it.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+// Loads that write local memory directly: 16 bytes, or 4, a lane, to `to` + lane * 16 (4).  As the builtin the compiler lets
+// every later read of local memory wait for them, whatever it reads: no load would be under way beside the products (4096 x
+// 4096 x 4096: 75 us that way).  There is no output register; what waits for them is wait_loads and the barrier behind it.
+__device__ __forceinline__ void load_quads(uint32_t to, uint32_t at, Rows rows, int offset)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(at), "s"(rows), "s"(offset)
+                 : "memory", "m0");
+}
+__device__ __forceinline__ void load_words(uint32_t to, uint32_t at, Rows rows, int offset)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(to), "v"(at), "s"(rows), "s"(offset)
+                 : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+__device__ __forceinline__ uint32_t local_address(const void* p)
+{
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
 
 template <int N>
 __device__ __forceinline__ void wait_loads()
 {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Writes a tile through local memory, so that whole lines of rows go out: lanes hold four n of 16 different m each (the tile of
+// 4096 x 4096 x 4096 that way took 62 us without a single load, of which 27 were its products).  The 16-byte pieces of row m
+// stand at place piece ^ (m % 16), or less where a row has fewer pieces.
+template <typename T, int BN, int BM, int TN, int TM, int WAVES>
+__device__ __forceinline__ void store_tile(uint8_t* lds, const v4f (&acc)[TN][TM], int wn, int wm, T* __restrict__ y, long m0,
+                                           long n0, const Fp8Shape& s, const float* __restrict__ bias, int relu)
+{
+    constexpr int PER = 16 / (int)sizeof(T), PIECES = BN / PER;      // elements of a piece, pieces of a row
+    constexpr int TURNS = PIECES < 16 ? PIECES : 16;
+    const int lane = threadIdx.x % kWave, row = lane % 16, piece = lane / 16;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TN; ++i) {
+        const int n = (wn * TN + i) * 16 + piece * 4;
+        v4f b = {0, 0, 0, 0};
+        if (bias) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (n0 + n + k < s.n) b[k] = bias[n0 + n + k];
+        }
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+            const int m = (wm * TM + j) * 16 + row;
+            Pack<T, 4> out;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float v = acc[i][j][k] + b[k];
+                if (relu) v = v > 0.0f ? v : 0.0f;
+                out.v[k] = (T)v;
+            }
+            *reinterpret_cast<Pack<T, 4>*>(lds + m * BN * sizeof(T) + ((n / PER) ^ (m % TURNS)) * 16 + n % PER * sizeof(T)) = out;
+        }
+    }
+    __syncthreads();
+    const bool whole = s.n % PER == 0 && ((uintptr_t)y & 15) == 0;
+#pragma unroll 4
+    for (int at = threadIdx.x; at < BM * PIECES; at += WAVES * kWave) {
+        const int m = at / PIECES, n = at % PIECES * PER;
+        if (m0 + m >= s.m || n0 + n >= s.n) continue;
+        const Pack<T, PER> v = *reinterpret_cast<const Pack<T, PER>*>(lds + m * BN * sizeof(T) + ((n / PER) ^ (m % TURNS)) * 16);
+        T* to = y + (m0 + m) * s.n + n0 + n;
+        if (whole) {
+            // past the caches: the workgroups of a launch store all at once (4096 x 4096 in bfloat16: 13 us, plain stores 19)
+            typedef uint32_t quad __attribute__((ext_vector_type(4)));
+            __builtin_nontemporal_store(*reinterpret_cast<const quad*>(&v), reinterpret_cast<quad*>(to));
+        } else {
+#pragma unroll
+            for (int k = 0; k < PER; ++k)
+                if (n0 + n + k < s.n) to[k] = v.v[k];
+        }
+    }
 }
 
 template <typename T, bool EXACT, int BN, int BM, int WN, int WM, int STAGES>
@@ -258,7 +340,10 @@ __global__ void __launch_bounds__(WN* WM* kWave, STAGES * (BN + BM) * kBlock > 8
     constexpr int WAVES = WN * WM, TN = BN / WN / 16, TM = BM / WM / 16;
     constexpr int WLOADS = BN / 8 / WAVES, LOADS = (BN + BM) / 8 / WAVES;     // loads of a wave and step: eight rows each
     constexpr int STAGE = (BN + BM) * kBlock;
+    constexpr int CHUNKS = (BN + BM) / 64;      // scale words: 64 rows to a load
+    constexpr int EACH = (CHUNKS + WAVES - 1) / WAVES;
     __shared__ __attribute__((aligned(128))) uint8_t lds[STAGES * STAGE];
+    __shared__ uint32_t scale[2][BN + BM];
 
     // Consecutive workgroups go to the eight dies in turn; a die's tiles are consecutive, in bands of four tiles of n, so that
     // its second-level cache holds what they share.
@@ -284,29 +369,33 @@ __global__ void __launch_bounds__(WN* WM* kWave, STAGES * (BN + BM) * kBlock > 8
         const int r = (wave + (i < WLOADS ? i : i - WLOADS) * WAVES) * 8 + lane / 8;
         from[i] = (uint32_t)(r * kp) + (uint32_t)(((lane % 8) ^ (lane / 8)) * 16);
     }
-    auto issue = [&](int step, int stage) {
+    // the scale words of W's rows, then of x's, 64 rows to a load
+    Rows scale_from[EACH];
+    const uint32_t scale_at = (uint32_t)(lane * s.words * 4);
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int group = i < WLOADS ? wave + i * WAVES : BN / 8 + wave + (i - WLOADS) * WAVES;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(i < WLOADS ? wres : xres, (LdsVoid*)(lds + stage * STAGE + group * 1024), 16,
-                                                     (int)from[i], step * kBlock, 0, 0);
+    for (int e = 0; e < EACH; ++e) {
+        const int chunk = wave + e * WAVES;
+        const bool of_w = chunk < BN / 64;
+        const long r = of_w ? n0 + chunk * 64 : m0 + (chunk - BN / 64) * 64, left = max((of_w ? s.n : s.m) - r, 0l);
+        scale_from[e] = rows_of((of_w ? ws : xs) + (left ? r : 0) * s.words, left * s.words * 4);
+    }
+    const uint32_t lds_at = local_address(lds), scales_at = local_address(scale);
+    auto load_rows = [&](int step, int stage, int i) {
+        const int group = i < WLOADS ? wave + i * WAVES : BN / 8 + wave + (i - WLOADS) * WAVES;
+        load_quads(lds_at + stage * STAGE + group * 1024, from[i], i < WLOADS ? wres : xres, step * kBlock);
+    };
+    // with the first of four steps, their scales; two words' scales have a place each
+    auto load_scales = [&](int step) {
+        if (step % 4 == 0) {
+#pragma unroll
+            for (int e = 0; e < EACH; ++e)
+                if (CHUNKS % WAVES == 0 || wave + e * WAVES < CHUNKS)
+                    load_words(scales_at + (step / 4 & 1) * (BN + BM) * 4 + (wave + e * WAVES) * 256, scale_at, scale_from[e],
+                               step / 4 * 4);
         }
     };
 
-    const uint32_t* wsp[TN];
-    const uint32_t* xsp[TM];
-#pragma unroll
-    for (int i = 0; i < TN; ++i) wsp[i] = ws + min(n0 + wn * TN * 16 + i * 16 + row, s.n - 1) * s.words;
-#pragma unroll
-    for (int j = 0; j < TM; ++j) xsp[j] = xs + min(m0 + wm * TM * 16 + j * 16 + row, s.m - 1) * s.words;
-    int we[TN], xe[TM], we_next[TN], xe_next[TM];
-    auto scales = [&](int word) {
-#pragma unroll
-        for (int i = 0; i < TN; ++i) we_next[i] = (int)wsp[i][word];
-#pragma unroll
-        for (int j = 0; j < TM; ++j) xe_next[j] = (int)xsp[j][word];
-    };
-
+    int we[TN] = {}, xe[TM] = {};
     v4f acc[TN][TM];
 #pragma unroll
     for (int i = 0; i < TN; ++i)
@@ -314,62 +403,67 @@ __global__ void __launch_bounds__(WN* WM* kWave, STAGES * (BN + BM) * kBlock > 8
         for (int j = 0; j < TM; ++j) acc[i][j] = v4f{0, 0, 0, 0};
 
     if (first < last) {
-        scales(first / 4);
 #pragma unroll
         for (int t = 0; t < STAGES - 1; ++t)
-            if (first + t < last) issue(first + t, t);
+            if (first + t < last) {
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) load_rows(first + t, t, i);
+                load_scales(first + t);
+            }
     }
     const uint32_t mine = (uint32_t)((row * kBlock) + ((piece ^ (row % 8)) * 16));
     const uint32_t wbase = (uint32_t)(wn * TN * 16 * kBlock) + mine, xbase = (uint32_t)((BN + wm * TM * 16) * kBlock) + mine;
     int stage = 0;
     for (int step = first; step < last; ++step) {
+        // this step's loads are the oldest; while later steps' follow them, those may stay under way
+        if (STAGES > 2 && step + STAGES - 2 < last) wait_loads<(STAGES - 2) * LOADS>();
+        else wait_loads<0>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");      // no access moves across the barrier
+        const int coming = step + STAGES - 1, coming_stage = stage == 0 ? STAGES - 1 : stage - 1;
+        if (coming < last) load_scales(coming);
+        const uint8_t* here = lds + stage * STAGE;
         if (step % 4 == 0) {
+            const uint32_t* words_here = scale[step / 4 & 1];
 #pragma unroll
-            for (int i = 0; i < TN; ++i) we[i] = we_next[i];
+            for (int i = 0; i < TN; ++i) we[i] = (int)words_here[(wn * TN + i) * 16 + row];
 #pragma unroll
-            for (int j = 0; j < TM; ++j) xe[j] = xe_next[j];
-            scales(min(step / 4 + 1, s.words - 1));
+            for (int j = 0; j < TM; ++j) xe[j] = (int)words_here[BN + (wm * TM + j) * 16 + row];
         } else {
 #pragma unroll
             for (int i = 0; i < TN; ++i) we[i] = (int)((uint32_t)we[i] >> 8);
 #pragma unroll
             for (int j = 0; j < TM; ++j) xe[j] = (int)((uint32_t)xe[j] >> 8);
         }
-        // this step's loads are the oldest; while later steps' follow them, those may stay under way
-        if (STAGES > 2 && step + STAGES - 2 < last) wait_loads<(STAGES - 2) * LOADS>();
-        else wait_loads<0>();
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");      // no access moves across the barrier
-        if (step + STAGES - 1 < last) issue(step + STAGES - 1, (stage + STAGES - 1) % STAGES);
-        const uint8_t* here = lds + stage * STAGE;
         v8i x[TM];
 #pragma unroll
         for (int j = 0; j < TM; ++j)
             x[j] = join(*reinterpret_cast<const v4i*>(here + xbase + j * 16 * kBlock),
                         *reinterpret_cast<const v4i*>(here + (xbase ^ 64u) + j * 16 * kBlock));
+        auto weights = [&](int i) {
+            return join(*reinterpret_cast<const v4i*>(here + wbase + i * 16 * kBlock),
+                        *reinterpret_cast<const v4i*>(here + (wbase ^ 64u) + i * 16 * kBlock));
+        };
+        v8i w = weights(0);
 #pragma unroll
         for (int i = 0; i < TN; ++i) {
-            const v8i w = join(*reinterpret_cast<const v4i*>(here + wbase + i * 16 * kBlock),
-                               *reinterpret_cast<const v4i*>(here + (wbase ^ 64u) + i * 16 * kBlock));
+            const v8i after = weights(i + 1 < TN ? i + 1 : i);
+            // a coming step's loads, a few at a time over the first half of the products
+            if (coming < last) {
+#pragma unroll
+                for (int l = i * 2 * LOADS / TN; l < (i + 1) * 2 * LOADS / TN && l < LOADS; ++l) load_rows(coming, coming_stage, l);
+            }
 #pragma unroll
             for (int j = 0; j < TM; ++j) acc[i][j] = block_product<EXACT>(w, we[i], x[j], xe[j], acc[i][j]);
+            w = after;
         }
         stage = stage + 1 == STAGES ? 0 : stage + 1;
     }
 
-#pragma unroll
-    for (int i = 0; i < TN; ++i) {
-        const long n = n0 + wn * TN * 16 + i * 16 + piece * 4;
-#pragma unroll
-        for (int j = 0; j < TM; ++j) {
-            const long m = m0 + wm * TM * 16 + j * 16 + row;
-            if (m >= s.m || n >= s.n) continue;
-            if (splits == 1) {
-                store_four(y, m, n, s, acc[i][j], bias, relu);
-            } else {
-                store_four(partial + split * s.m * s.n, m, n, s, acc[i][j], nullptr, 0);
-            }
-        }
+    if (splits == 1) {
+        store_tile<T, BN, BM, TN, TM, WAVES>(lds, acc, wn, wm, y, m0, n0, s, bias, relu);
+    } else if constexpr (BN * BM * 4 <= STAGES * STAGE) {
+        store_tile<float, BN, BM, TN, TM, WAVES>(lds, acc, wn, wm, partial + split * s.m * s.n, m0, n0, s, nullptr, 0);
     }
 }
 
@@ -411,7 +505,7 @@ Tiling tiling_of(const Fp8Shape& s, bool exact)
     if (!exact && tiles(256) >= 192) t.size = 256;
     else if (tiles(128) >= 192) t.size = 128;
     const long count = tiles(t.size);
-    if (count < 256) {
+    if (count < 256 && t.size < 256) {
         long splits = 512 / count;
         if (splits > s.words / 2) splits = s.words / 2;
         if (splits > kSplitsMost) splits = kSplitsMost;
@@ -495,7 +589,7 @@ int product(const uint8_t* xq, const uint8_t* xs, const uint8_t* wq, const uint8
     const Tiling t = tiling_of(s, EXACT);
     if constexpr (!EXACT)
         if (t.size == 256)
-            return launch_tiles<T, EXACT, 256, 256, 2, 4, 2>(xq, xs, wq, ws, bias, y, partial, s, relu, t.splits, st);
+                        return launch_tiles<T, EXACT, 256, 256, 2, 4, 2>(xq, xs, wq, ws, bias, y, partial, s, relu, t.splits, st);
     if (t.size == 128) return launch_tiles<T, EXACT, 128, 128, 2, 2, 2>(xq, xs, wq, ws, bias, y, partial, s, relu, t.splits, st);
     return launch_tiles<T, EXACT, 64, 64, 2, 2, 4>(xq, xs, wq, ws, bias, y, partial, s, relu, t.splits, st);
 }
