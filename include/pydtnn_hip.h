@@ -449,13 +449,14 @@ int pydtnn_hip_bn_training_bwd_f64(const double *dy, const double *xn, const dou
  *   backward: from dy, x and the forward's mean and inv_std: dgamma, dbeta (channels) and, unless it is NULL, dx.
  *             Where the activation is PYDTNN_HIP_ACT_RELU, dy counts where z, computed from these inputs, is positive.
  * Sums are taken in a fixed order.  Outputs may not overlap inputs.  channels has to be a multiple of groups; pixels and
- * channels are at most 2^30 (PYDTNN_HIP_ERR_UNSUPPORTED).  Workspace: pydtnn_hip_gn_workspace_bytes(...) with the same
- * extents; backward = 0 or 1. */
+ * channels are at most 2^30 (PYDTNN_HIP_ERR_UNSUPPORTED).  Workspace, aligned to 16 bytes: pydtnn_hip_gn_workspace_bytes(...)
+ * with the same extents; backward = 0 or 1; aligned: whether x, y (x, dy and dx) start on multiples of 16 bytes.  Where the
+ * forward pass needs none (0) it may be NULL. */
 #define PYDTNN_HIP_ACT_IDENTITY 0
 #define PYDTNN_HIP_ACT_RELU 1
 #define PYDTNN_HIP_ACT_SILU 2
 size_t pydtnn_hip_gn_workspace_bytes(int dtype, int nhwc, int backward, long images, long channels, long pixels,
-                                     long groups);
+                                     long groups, int aligned);
 int pydtnn_hip_gn_forward(int dtype, int nhwc, const void *x, const void *gamma, const void *beta, void *y, void *mean,
                           void *inv_std, long images, long channels, long pixels, long groups, double eps,
                           int activation, void *workspace, size_t workspace_bytes, void *stream);

@@ -44,7 +44,46 @@ __device__ __forceinline__ int scale_byte(uint32_t amax)
     return e < 0 ? 0 : e;
 }
 
-// One wave takes four blocks of a row, 16 lanes a block, eight elements a lane.
+struct Eight {
+    uint2 q;
+    int byte;
+};
+
+// Eight elements c .. c + 7 of a row, by one of the 16 lanes that have a block: their e4m3 values and the block's scale byte.
+template <typename T, bool PACKED>
+__device__ __forceinline__ Eight quantize_eight(const T* __restrict__ row, long c, long k)
+{
+    float v[8];
+    if (PACKED && c + 8 <= k) {
+        const Pack<T, 8> p = *reinterpret_cast<const Pack<T, 8>*>(row + c);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (float)p.v[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = c + j < k ? (float)row[c + j] : 0.0f;
+    }
+    uint32_t amax = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, o, kWave));
+    Eight e;
+    if (amax < 0x7f800000u) {
+        e.byte = scale_byte(amax);
+        const float inverse = __uint_as_float((uint32_t)(254 - e.byte) << 23);      // 2^-(byte - 127), byte <= 247
+        int a = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inverse, v[1] * inverse, 0, false);
+        int b = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * inverse, v[5] * inverse, 0, false);
+        a = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inverse, v[3] * inverse, a, true);
+        b = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * inverse, v[7] * inverse, b, true);
+        e.q = make_uint2((uint32_t)a, (uint32_t)b);
+    } else {      // an infinity or a NaN
+        e.byte = 127;
+        e.q = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+    }
+    return e;
+}
+
+// One wave takes four blocks of a row, 16 lanes a block.
 template <typename T, bool PACKED>
 __global__ void __launch_bounds__(kT) quantize_fp8_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
                                                           uint32_t* __restrict__ scales, long rows, long k, int blocks,
@@ -55,40 +94,12 @@ __global__ void __launch_bounds__(kT) quantize_fp8_kernel(const T* __restrict__ 
     const long row = item / words;
     const int lane = threadIdx.x % kWave;
     const long c = (item % words) * 4 * kBlock + lane * 8;
-    float v[8];
-    if (PACKED && c + 8 <= k) {
-        const Pack<T, 8> p = *reinterpret_cast<const Pack<T, 8>*>(x + row * k + c);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = (float)p.v[j];
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = c + j < k ? (float)x[row * k + c + j] : 0.0f;
-    }
-    uint32_t amax = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7fffffffu);
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, o, kWave));
-    const bool finite = amax < 0x7f800000u;
-    const bool real = c / kBlock < blocks;
-    const int byte = finite && real ? scale_byte(amax) : 127;
-    const float inverse = __uint_as_float((uint32_t)(254 - byte) << 23);      // 2^-(byte - 127), byte <= 247
-    if (real) {
-        uint2 out;
-        if (finite) {
-            int a = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inverse, v[1] * inverse, 0, false);
-            int b = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * inverse, v[5] * inverse, 0, false);
-            a = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inverse, v[3] * inverse, a, true);
-            b = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * inverse, v[7] * inverse, b, true);
-            out = make_uint2((uint32_t)a, (uint32_t)b);
-        } else {
-            out = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
-        }
-        *reinterpret_cast<uint2*>(q + row * blocks * kBlock + c) = out;
-    }
+    Eight e = quantize_eight<T, PACKED>(x + row * k, c, k);
+    if (c / kBlock < blocks) *reinterpret_cast<uint2*>(q + row * blocks * kBlock + c) = e.q;
+    else e.byte = 127;
     uint32_t word = 0;
 #pragma unroll
-    for (int b = 0; b < 4; ++b) word |= (uint32_t)__shfl(byte, b * 16, kWave) << (8 * b);
+    for (int b = 0; b < 4; ++b) word |= (uint32_t)__shfl(e.byte, b * 16, kWave) << (8 * b);
     if (lane == 0) scales[item] = word;
 }
 
@@ -143,54 +154,66 @@ __device__ __forceinline__ void store_four(T* y, long m, long n, const Fp8Shape&
         if (n + i < s.n) to[i] = finish<T>(v[i], bias, n + i, relu);
 }
 
+// A buffer resource over rows from `base`: what is read behind the last byte is zero.
+typedef __amdgpu_buffer_rsrc_t Rows;
+__device__ __forceinline__ Rows rows_of(const void* base, long bytes)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)(uint32_t)min(bytes, 0xffffffffl), 0x00020000);
+}
+
+// The same as the four words that inline assembly takes.
+typedef v4i RowsWords;
+__device__ __forceinline__ RowsWords rows_words(const void* base, long bytes)
+{
+    return RowsWords{(int)(uint32_t)(uintptr_t)base, (int)((uintptr_t)base >> 32), (int)(uint32_t)min(bytes, 0xffffffffl),
+                     0x00020000};
+}
+
 // ---------------------------------------------------------------------------------------------- few rows
-// Up to 16 * MT rows of x: bound by reading the weights, each of which is used for those rows only.  A workgroup takes 16
-// rows of the weights; its waves take the words of four blocks in turn, with the next word's operands on their way while
+// Up to 16 rows of x: bound by reading the weights, each of which is used for those rows only.  A workgroup takes 16 rows
+// of the weights; its waves take the words of four blocks in turn, with the next word's operands on their way while
 // the present one's are multiplied, and join their sums in local memory, in the order of the waves.  The weights are the
 // first operand, so that a lane ends with four consecutive n of one m.
-constexpr int kFewWaves = 8;
+//
+// Where local memory holds all of x (kFewLocal bytes), every workgroup quantises it for itself, while its first weights
+// are on their way: one launch instead of two.  Otherwise x comes quantised.
+constexpr int kFewWaves = 8, kFewLocal = 32 * 1024;
 
 __device__ __forceinline__ v8i join(v4i a, v4i b)
 {
     return v8i{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
-template <int MT>
+// A word of four blocks of 16 rows: a lane's two pieces of each block, and the four scale bytes.  (What it reads of blocks
+// behind the last of a row is not used.)
 struct WordOfBlocks {
-    v4i w[4][2], x[MT][4][2];
-    int we, xe[MT];
+    v4i q[4][2];
+    int e;
 
-    __device__ __forceinline__ void load(const v4i* wp, const v4i* const (&xp)[MT], const uint32_t* wsp,
-                                         const uint32_t* const (&xsp)[MT], int word, int blocks)
+    // `at`: a lane's offset in bytes, of its row and piece; `scale_at`: that of its row's scales
+    __device__ __forceinline__ void load(Rows rows, int at, Rows scales, int scale_at, int word)
     {
-        we = (int)wsp[word];
-#pragma unroll
-        for (int t = 0; t < MT; ++t) xe[t] = (int)xsp[t][word];
+        e = __builtin_amdgcn_raw_buffer_load_b32(scales, scale_at, word * 4, 0);
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-            const long at = (long)min(word * 4 + b, blocks - 1) * (kBlock / 16);
-            w[b][0] = wp[at], w[b][1] = wp[at + 4];
-#pragma unroll
-            for (int t = 0; t < MT; ++t) x[t][b][0] = xp[t][at], x[t][b][1] = xp[t][at + 4];
+            q[b][0] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rows, at, (word * 4 + b) * kBlock, 0));
+            q[b][1] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rows, at + 64, (word * 4 + b) * kBlock, 0));
         }
     }
-
-    template <bool EXACT>
-    __device__ __forceinline__ void multiply(int word, int blocks, v4f (&acc)[MT]) const
+    __device__ __forceinline__ void load(const uint8_t* row, const uint8_t* scales, int word)
     {
+        e = *reinterpret_cast<const int*>(scales + word * 4);
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-            if (word * 4 + b >= blocks) break;
-#pragma unroll
-            for (int t = 0; t < MT; ++t)
-                acc[t] = block_product<EXACT>(join(w[b][0], w[b][1]), we >> (8 * b), join(x[t][b][0], x[t][b][1]),
-                                              xe[t] >> (8 * b), acc[t]);
+            q[b][0] = *reinterpret_cast<const v4i*>(row + (word * 4 + b) * kBlock);
+            q[b][1] = *reinterpret_cast<const v4i*>(row + (word * 4 + b) * kBlock + 64);
         }
     }
 };
 
-template <typename T, int MT>
-__global__ void __launch_bounds__(kFewWaves* kWave) matmul_fp8_few_kernel(const uint8_t* __restrict__ xq,
+template <typename T, int DEPTH, bool LOCAL, bool PACKED>
+__global__ void __launch_bounds__(kFewWaves* kWave) matmul_fp8_few_kernel(const T* __restrict__ x,
+                                                                          const uint8_t* __restrict__ xq,
                                                                           const uint32_t* __restrict__ xs,
                                                                           const uint8_t* __restrict__ wq,
                                                                           const uint32_t* __restrict__ ws,
@@ -198,41 +221,68 @@ __global__ void __launch_bounds__(kFewWaves* kWave) matmul_fp8_few_kernel(const 
                                                                           Fp8Shape s, int relu)
 {
     constexpr bool EXACT = sizeof(T) == 4;
-    __shared__ v4f part[kFewWaves][MT][kWave];
-    const int lane = threadIdx.x % kWave, row = lane % 16, piece = lane / 16, wave = threadIdx.x / kWave;
-    const long n0 = (long)blockIdx.x * 16;
-    const long wr = min(n0 + row, s.n - 1), kp = (long)s.blocks * kBlock;
-    const v4i* wp = reinterpret_cast<const v4i*>(wq + wr * kp) + piece;
-    const uint32_t* wsp = ws + wr * s.words;
-    const v4i* xp[MT];
-    const uint32_t* xsp[MT];
-    v4f acc[MT];
+    __shared__ v4f part[kFewWaves][kWave];
+    // a row of x and its scale words; 16 bytes more than its values, so that rows start on different banks
+    __shared__ __attribute__((aligned(16))) uint8_t local[LOCAL ? kFewLocal + 4 * kBlock : 16];      // (the last word's end)
+    const int lane = threadIdx.x % kWave, row = lane % 16, piece = lane / 16;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const long n0 = (long)blockIdx.x * 16, kp = (long)s.blocks * kBlock;
+    const Rows wrows = rows_of(wq + n0 * kp, (s.n - n0) * kp), wscales = rows_of(ws + n0 * s.words, (s.n - n0) * s.words * 4);
+    const int at = (int)(row * kp) + piece * 16, scale_at = row * s.words * 4;
+    v4f acc = {0, 0, 0, 0};
+    // The wave's words are wave, wave + kFewWaves, ...; DEPTH - 1 of them are on their way while one is multiplied.  They stand
+    // in places of their own in turn: a copy from one place to another would wait for its loads.
+    const int mine = s.words > wave ? (s.words - wave + kFewWaves - 1) / kFewWaves : 0;
+    auto word_of = [&](int i) { return wave + i * kFewWaves; };
+    WordOfBlocks w[DEPTH], v[LOCAL ? 1 : DEPTH];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const long xr = min((long)t * 16 + row, s.m - 1);
-        xp[t] = reinterpret_cast<const v4i*>(xq + xr * kp) + piece;
-        xsp[t] = xs + xr * s.words;
-        acc[t] = v4f{0, 0, 0, 0};
-    }
-    // two words in turn, without a copy from one to the other: a copy would wait for the loads
-    WordOfBlocks<MT> even, odd;
-    if (wave < s.words) even.load(wp, xp, wsp, xsp, wave, s.blocks);
-    for (int word = wave; word < s.words; word += 2 * kFewWaves) {
-        odd.load(wp, xp, wsp, xsp, min(word + kFewWaves, s.words - 1), s.blocks);
-        even.template multiply<EXACT>(word, s.blocks, acc);
-        if (word + kFewWaves >= s.words) break;
-        even.load(wp, xp, wsp, xsp, min(word + 2 * kFewWaves, s.words - 1), s.blocks);
-        odd.template multiply<EXACT>(word + kFewWaves, s.blocks, acc);
-    }
+    for (int d = 0; d < DEPTH - 1; ++d)
+        if (d < mine) w[d].load(wrows, at, wscales, scale_at, word_of(d));
+    const long stride = kp + 16 + (s.words * 4 + 15) / 16 * 16;
+    // rows behind the last are that one again in local memory, zeros otherwise
+    const uint8_t* xlocal = local + min((long)row, s.m - 1) * stride;
+    const Rows xrows = rows_of(xq, LOCAL ? 0 : s.m * kp), xscales = rows_of(xs, LOCAL ? 0 : s.m * s.words * 4);
+    if constexpr (LOCAL) {
+        for (int item = wave; item < s.m * s.words; item += kFewWaves) {
+            const int r = item / s.words, word = item % s.words, c = word * 4 * kBlock + lane * 8;
+            const Eight e = quantize_eight<T, PACKED>(x + (long)r * s.k, c, s.k);
+            if (c < kp) {
+                *reinterpret_cast<uint2*>(local + r * stride + c) = e.q;
+                if (lane % 16 == 0) local[r * stride + kp + 16 + c / kBlock] = (uint8_t)e.byte;
+            }
+        }
+        __syncthreads();
+    } else {
 #pragma unroll
-    for (int t = 0; t < MT; ++t) part[wave][t][lane] = acc[t];
+        for (int d = 0; d < DEPTH - 1; ++d)
+            if (d < mine) v[d].load(xrows, at, xscales, scale_at, word_of(d));
+    }
+    for (int done = 0; done < mine; done += DEPTH) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            if (done + d >= mine) break;
+            const int ahead = word_of(done + d + DEPTH - 1), word = word_of(done + d);
+            const bool more = done + d + DEPTH - 1 < mine;
+            if (more) w[(d + DEPTH - 1) % DEPTH].load(wrows, at, wscales, scale_at, ahead);
+            if constexpr (LOCAL) v[0].load(xlocal + piece * 16, xlocal + kp + 16, word);
+            else if (more) v[(d + DEPTH - 1) % DEPTH].load(xrows, at, xscales, scale_at, ahead);
+            const WordOfBlocks& here = v[LOCAL ? 0 : d];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                if (word * 4 + b >= s.blocks) break;
+                acc = block_product<EXACT>(join(w[d].q[b][0], w[d].q[b][1]), w[d].e >> (8 * b), join(here.q[b][0], here.q[b][1]),
+                                           here.e >> (8 * b), acc);
+            }
+        }
+    }
+    part[wave][lane] = acc;
     __syncthreads();
-    for (int t = wave; t < MT; t += kFewWaves) {
-        v4f sum = part[0][t][lane];
+    if (wave > 0) return;
+    v4f sum = part[0][lane];
 #pragma unroll
-        for (int v = 1; v < kFewWaves; ++v) sum += part[v][t][lane];
-        if (t * 16 + row < s.m && n0 + piece * 4 < s.n) store_four(y, (long)t * 16 + row, n0 + piece * 4, s, sum, bias, relu);
-    }
+    for (int k = 1; k < kFewWaves; ++k) sum += part[k][lane];
+    const long n = n0 + piece * 4;
+    if (row < s.m && n < s.n) store_four(y, (long)row, n, s, sum, bias, relu);
 }
 
 // ---------------------------------------------------------------------------------------------- tiles
@@ -241,26 +291,18 @@ __global__ void __launch_bounds__(kFewWaves* kWave) matmul_fp8_few_kernel(const 
 // eight 16-byte pieces of a row r stand at place piece ^ (r % 8), so that the sixteen rows that a fragment reads at once fall
 // on different banks; the loads' lanes pick their pieces accordingly, and since a lane's two pieces of a block are any two,
 // as long as both operands take the same, a lane takes pieces p and p + 4.
-typedef v4i Rows;      // a buffer resource
-
-// Rows from `base`; those behind the last byte read as zeros.
-__device__ __forceinline__ Rows rows_of(const void* base, long bytes)
-{
-    return Rows{(int)(uint32_t)(uintptr_t)base, (int)((uintptr_t)base >> 32), (int)(uint32_t)min(bytes, 0xffffffffl), 0x00020000};
-}
-
 // m0 is set here and nowhere else; the compiler warns that it reserves it.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 // Loads that write local memory directly: 16 bytes, or 4, a lane, to `to` + lane * 16 (4).  As the builtin the compiler lets
 // every later read of local memory wait for them, whatever it reads: no load would be under way beside the products (4096 x
 // 4096 x 4096: 75 us that way).  There is no output register; what waits for them is wait_loads and the barrier behind it.
-__device__ __forceinline__ void load_quads(uint32_t to, uint32_t at, Rows rows, int offset)
+__device__ __forceinline__ void load_quads(uint32_t to, uint32_t at, RowsWords rows, int offset)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(at), "s"(rows), "s"(offset)
                  : "memory", "m0");
 }
-__device__ __forceinline__ void load_words(uint32_t to, uint32_t at, Rows rows, int offset)
+__device__ __forceinline__ void load_words(uint32_t to, uint32_t at, RowsWords rows, int offset)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(to), "v"(at), "s"(rows), "s"(offset)
                  : "memory", "m0");
@@ -362,7 +404,7 @@ __global__ void __launch_bounds__(WN* WM* kWave, STAGES * (BN + BM) * kBlock > 8
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int row = lane % 16, piece = lane / 16, wn = wave % WN, wm = wave / WN;
     const long kp = (long)s.blocks * kBlock;
-    const Rows wres = rows_of(wq + n0 * kp, (s.n - n0) * kp), xres = rows_of(xq + m0 * kp, (s.m - m0) * kp);
+    const RowsWords wres = rows_words(wq + n0 * kp, (s.n - n0) * kp), xres = rows_words(xq + m0 * kp, (s.m - m0) * kp);
     uint32_t from[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
@@ -370,14 +412,14 @@ __global__ void __launch_bounds__(WN* WM* kWave, STAGES * (BN + BM) * kBlock > 8
         from[i] = (uint32_t)(r * kp) + (uint32_t)(((lane % 8) ^ (lane / 8)) * 16);
     }
     // the scale words of W's rows, then of x's, 64 rows to a load
-    Rows scale_from[EACH];
+    RowsWords scale_from[EACH];
     const uint32_t scale_at = (uint32_t)(lane * s.words * 4);
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
         const int chunk = wave + e * WAVES;
         const bool of_w = chunk < BN / 64;
         const long r = of_w ? n0 + chunk * 64 : m0 + (chunk - BN / 64) * 64, left = max((of_w ? s.n : s.m) - r, 0l);
-        scale_from[e] = rows_of((of_w ? ws : xs) + (left ? r : 0) * s.words, left * s.words * 4);
+        scale_from[e] = rows_words((of_w ? ws : xs) + (left ? r : 0) * s.words, left * s.words * 4);
     }
     const uint32_t lds_at = local_address(lds), scales_at = local_address(scale);
     auto load_rows = [&](int step, int stage, int i) {
@@ -489,11 +531,14 @@ bool shape_of(Fp8Shape* s, long m, long n, long k)
 size_t q_bytes(const Fp8Shape& s) { return (size_t)s.m * s.blocks * kBlock; }
 size_t scale_bytes(const Fp8Shape& s) { return ((size_t)s.m * s.words * 4 + 15) / 16 * 16; }
 
-constexpr long kFewRows = 32;
+constexpr long kFewRows = 16;
 constexpr int kSplitsMost = 16;
 
-// Tiles of `size` by `size`, and how many pieces k is cut into: where there are fewer tiles than 256 compute units, until
-// there are about twice as many, each with at least four words of four blocks.
+// Tiles of `size` by `size`: the largest that are about enough for 256 compute units (512 x 4096 x 4096 in bfloat16: 23 us with
+// 256 tiles of 128 by 128 ... 4096 x 4096 x 4096: 73 us with 256 by 256, 86 with 128 by 128).  Where there are fewer, k is cut
+// into `splits` pieces of at least two words of four blocks, a workgroup each, as far as there are units for them (777 x 2049 x
+// 1003 in float16: 15 us with 208 workgroups, 20 with twice as many, whose results have to be joined; 64 x 25088 x 4096: 37
+// and 41).
 struct Tiling {
     int size, splits;
 };
@@ -506,12 +551,18 @@ Tiling tiling_of(const Fp8Shape& s, bool exact)
     else if (tiles(128) >= 192) t.size = 128;
     const long count = tiles(t.size);
     if (count < 256 && t.size < 256) {
-        long splits = 512 / count;
-        if (splits > s.words / 2) splits = s.words / 2;
+        long splits = 256 / count;
+                if (splits > s.words / 2) splits = s.words / 2;
         if (splits > kSplitsMost) splits = kSplitsMost;
         if (splits > 1) t.splits = (int)splits;
     }
     return t;
+}
+
+// Whether a workgroup of the few rows' kernel holds all of x: values, scales and 16 bytes a row.
+bool few_local(const Fp8Shape& s)
+{
+    return s.m <= kFewRows && s.m * ((long)s.blocks * kBlock + 16 + (s.words * 4 + 15) / 16 * 16) <= kFewLocal;
 }
 
 size_t partial_bytes(const Fp8Shape& s, bool exact)
@@ -569,27 +620,28 @@ int launch_tiles(const uint8_t* xq, const uint8_t* xs, const uint8_t* wq, const 
 }
 
 template <typename T>
-int product(const uint8_t* xq, const uint8_t* xs, const uint8_t* wq, const uint8_t* ws, const float* bias, T* y, float* partial,
-            const Fp8Shape& s, int relu, hipStream_t st)
+int product(const T* x, const uint8_t* xq, const uint8_t* xs, const uint8_t* wq, const uint8_t* ws, const float* bias, T* y,
+            float* partial, const Fp8Shape& s, int relu, hipStream_t st)
 {
     constexpr bool EXACT = sizeof(T) == 4;
     if (s.m <= kFewRows) {
         const long blocks = (s.n + 15) / 16;
         if (blocks * kFewWaves * kWave >= (1l << 32)) return PYDTNN_HIP_ERR_UNSUPPORTED;
-        auto few = [&](auto tiles) {
-            hipLaunchKernelGGL((matmul_fp8_few_kernel<T, decltype(tiles)::value>), dim3((unsigned)blocks),
-                               dim3(kFewWaves * kWave), 0, st, xq, (const uint32_t*)xs, wq, (const uint32_t*)ws, bias, y, s,
-                               relu);
+        auto few = [&](auto depth, auto local, auto packed) {
+            hipLaunchKernelGGL((matmul_fp8_few_kernel<T, decltype(depth)::value, decltype(local)::value, decltype(packed)::value>),
+                               dim3((unsigned)blocks), dim3(kFewWaves * kWave), 0, st, x, xq, (const uint32_t*)xs, wq,
+                               (const uint32_t*)ws, bias, y, s, relu);
         };
-        if (s.m <= 16) few(std::integral_constant<int, 1>());
-        else few(std::integral_constant<int, 2>());
+        if (!few_local(s)) few(std::integral_constant<int, 2>(), std::false_type(), std::false_type());
+        else if (aligned16(x) && s.k % 8 == 0) few(std::integral_constant<int, 2>(), std::true_type(), std::true_type());
+        else few(std::integral_constant<int, 2>(), std::true_type(), std::false_type());
         HIP_RETURN_IF_LAUNCH_FAILED();
         return PYDTNN_HIP_OK;
     }
     const Tiling t = tiling_of(s, EXACT);
     if constexpr (!EXACT)
         if (t.size == 256)
-                        return launch_tiles<T, EXACT, 256, 256, 2, 4, 2>(xq, xs, wq, ws, bias, y, partial, s, relu, t.splits, st);
+            return launch_tiles<T, EXACT, 256, 256, 2, 4, 2>(xq, xs, wq, ws, bias, y, partial, s, relu, t.splits, st);
     if (t.size == 128) return launch_tiles<T, EXACT, 128, 128, 2, 2, 2>(xq, xs, wq, ws, bias, y, partial, s, relu, t.splits, st);
     return launch_tiles<T, EXACT, 64, 64, 2, 2, 4>(xq, xs, wq, ws, bias, y, partial, s, relu, t.splits, st);
 }
@@ -617,7 +669,7 @@ size_t pydtnn_hip_matmul_fp8_workspace_bytes(int dtype, long m, long n, long k)
 {
     Fp8Shape s;
     if (!shape_of(&s, m, n, k) || too_large(m, n, k)) return 0;
-    return q_bytes(s) + scale_bytes(s) + partial_bytes(s, dtype == kDtypeF32);
+    return few_local(s) ? 0 : q_bytes(s) + scale_bytes(s) + partial_bytes(s, dtype == kDtypeF32);
 }
 
 int pydtnn_hip_matmul_fp8(int dtype, const void* x, long m, long k, const uint8_t* wq, const uint8_t* wscales, long n,
@@ -628,17 +680,17 @@ int pydtnn_hip_matmul_fp8(int dtype, const void* x, long m, long k, const uint8_
     if (!aligned16(wq) || ((uintptr_t)wscales & 3)) return PYDTNN_HIP_ERR_INVALID;
     if (too_large(m, n, k)) return PYDTNN_HIP_ERR_UNSUPPORTED;
     if (dtype == kDtypeF64) return PYDTNN_HIP_ERR_INVALID;
-    if (!workspace || !aligned16(workspace) || workspace_bytes < pydtnn_hip_matmul_fp8_workspace_bytes(dtype, m, n, k))
-        return PYDTNN_HIP_ERR_WORKSPACE;
+    const size_t need = pydtnn_hip_matmul_fp8_workspace_bytes(dtype, m, n, k);
+    if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return PYDTNN_HIP_ERR_WORKSPACE;
     return with_fp8_input(dtype, [&](auto t) {
         using T = decltype(t);
         const hipStream_t st = convint::as_stream(stream);
         uint8_t* xq = static_cast<uint8_t*>(workspace);
-        uint8_t* xs = xq + q_bytes(s);
-        float* partial = reinterpret_cast<float*>(xs + scale_bytes(s));
-        const int rc = quantize<T>((const T*)x, m, k, xq, xs, st);
+        uint8_t* xs = need ? xq + q_bytes(s) : nullptr;
+        float* partial = need ? reinterpret_cast<float*>(xs + scale_bytes(s)) : nullptr;
+        const int rc = need ? quantize<T>((const T*)x, m, k, xq, xs, st) : PYDTNN_HIP_OK;
         if (rc != PYDTNN_HIP_OK) return rc;
-        return product<T>(xq, xs, wq, wscales, bias, (T*)y, partial, s, relu, st);
+        return product<T>((const T*)x, xq, xs, wq, wscales, bias, (T*)y, partial, s, relu, st);
     });
 }
 

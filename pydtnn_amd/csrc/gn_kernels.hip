@@ -897,9 +897,9 @@ GnLast last_shape(long images, int channels, int pixels, int groups, int v)
 
 // Where one kernel can hold a slab of an image in the registers of `threads` threads, `packs` packs of 16 bytes each (of x,
 // and in the backward pass as many of dy): the smallest slab of whole groups whose rows have at least `line` bytes, or all
-// channels.
-bool whole_shape(GnLast* g, long images, int channels, int pixels, int groups, int v, int size, int line, int threads,
-                 int packs)
+// channels; at most `most` of them.
+bool whole_shape(GnLast* g, long images, int channels, int pixels, int groups, int v, int size, int line, long most,
+                 int threads, int packs)
 {
     if (v * size != 16) return false;
     const int cg = channels / groups;
@@ -913,7 +913,7 @@ bool whole_shape(GnLast* g, long images, int channels, int pixels, int groups, i
         *g = GnLast{images, pixels, channels, groups, cg, sg, width, groups / sg, tx, threads / tx, 1, pixels,
                     images * (groups / sg), 1, 1, {}};
         set_joins(g, threads, v);
-        return true;
+        return g->pieces <= most && (g->pieces + 8) * threads < (1l << 32);      // (a launch counts its threads in 32 bits)
     }
     return false;
 }
@@ -928,29 +928,53 @@ int check(long images, long channels, long pixels, long groups)
 
 int size_of(int dtype) { return dtype == kDtypeF64 ? 8 : dtype == kDtypeF32 ? 4 : 2; }
 
-struct Pieces {
-    long moments, sums;      // moments of the forward pass, channel sums (of each kind) of the backward pass
-    size_t wide;
-};
-
-// `v` is a pack that the tensors' addresses allow or a larger one: pieces depend on it, so the query asks for both.
-Pieces pieces_of(int dtype, int nhwc, long images, int channels, int pixels, int groups, int v)
+// Calls launch(line, most, threads, packs) for the ways to hold a slab, the better first, until one fits: 256 threads before more
+// (several workgroups to a compute unit, whose loads and stores overlap) and whole lines of 128 bytes before half lines
+// (forward 64 x 14 x 14 x 1024 in float32: 19 us with lines, 22 with half lines).  The largest workgroup has a compute unit
+// to itself and is taken where one round of them does it all: forward 56 x 56 x 256 in float32 takes 22 us against 30 in two
+// passes for 16 images (256 slabs), 103 against 102 for 64.
+template <int FEW, int SOME_THREADS, int SOME, int MANY_THREADS, int MANY, typename F>
+bool hold_slabs(F launch)
 {
-    Pieces p;
-    p.wide = dtype == kDtypeF64 ? 8 : 4;
-    if (nhwc) {
-        const GnLast g = last_shape(images, channels, pixels, groups, v);
-        p.moments = images * groups * g.splits;
-        p.sums = images * g.splits * channels;
-    } else {
-        p.moments = p.sums = images * channels;
-    }
-    return p;
+    using std::integral_constant;
+    for (int line = 128; line >= 64; line /= 2)
+        if (launch(line, 1l << 40, integral_constant<int, 256>(), integral_constant<int, FEW>()) ||
+            launch(line, 1l << 40, integral_constant<int, SOME_THREADS>(), integral_constant<int, SOME>()))
+            return true;
+    for (int line = 128; line >= 64; line /= 2)
+        if (launch(line, 256l, integral_constant<int, MANY_THREADS>(), integral_constant<int, MANY>())) return true;
+    return false;
 }
 
-size_t workspace_of(const Pieces& p, long images, int groups, bool backward)
+// SHORT: packs of eight 16-bit values, which leave room for fewer threads.
+template <bool SHORT, typename F>
+bool hold_forward(F launch)
 {
-    return (backward ? 2 * p.sums + 2 * images * groups : 2 * p.moments) * p.wide;
+    return hold_slabs<4, 256, 16, SHORT ? 512 : 1024, SHORT ? 24 : 16>(launch);
+}
+
+template <bool SHORT, typename F>
+bool hold_backward(F launch)
+{
+    return hold_slabs<4, SHORT ? 256 : 512, 8, SHORT ? 512 : 1024, SHORT ? 12 : 8>(launch);
+}
+
+size_t workspace_bytes_of(int dtype, bool nhwc, bool backward, long images, int channels, int pixels, int groups, bool aligned)
+{
+    const int size = size_of(dtype), wide = dtype == kDtypeF64 ? 8 : 4;
+    const int v = aligned ? pack_of(size, channels, channels / groups) : 1;
+    long moments = images * channels, sums = images * channels;      // pieces of groups, of channels
+    if (nhwc) {
+        auto fits = [&](int line, long most, auto threads, auto packs) {
+            GnLast g;
+            return whole_shape(&g, images, channels, pixels, groups, v, size, line, most, threads, packs);
+        };
+        if (!backward && (size == 2 ? hold_forward<true>(fits) : hold_forward<false>(fits))) return 0;
+        const GnLast g = last_shape(images, channels, pixels, groups, v);
+        moments = images * groups * g.splits;
+        sums = images * channels * g.splits;
+    }
+    return (size_t)(backward ? 2 * sums + 2 * images * groups : 2 * moments) * wide;
 }
 
 template <typename F>
@@ -980,24 +1004,6 @@ bool too_many(long blocks) { return blocks * kT >= (1l << 32); }      // a launc
 // Planes of fewer pixels than this go to a wave each.
 constexpr int kPlaneOfGroup = 1024;
 
-// Calls launch(line, threads, packs) for the ways to hold a slab, the better first, until one fits: 256 threads before more
-// (several workgroups to a compute unit, whose loads and stores overlap) and whole lines of 128 bytes before half lines
-// (forward 64 x 14 x 14 x 1024 in float32: 19 us with lines, 22 with half lines).  The largest workgroup has a compute unit
-// to itself and is taken where one round of them does it all: forward 56 x 56 x 256 in float32 takes 22 us against 30 in two
-// passes for 16 images (256 slabs), 103 against 102 for 64.
-template <int FEW, int SOME_THREADS, int SOME, int MANY_THREADS, int MANY, typename F>
-bool hold_slabs(F launch)
-{
-    using std::integral_constant;
-    for (int line = 128; line >= 64; line /= 2)
-        if (launch(line, 1l << 40, integral_constant<int, 256>(), integral_constant<int, FEW>()) ||
-            launch(line, 1l << 40, integral_constant<int, SOME_THREADS>(), integral_constant<int, SOME>()))
-            return true;
-    for (int line = 128; line >= 64; line /= 2)
-        if (launch(line, 256l, integral_constant<int, MANY_THREADS>(), integral_constant<int, MANY>())) return true;
-    return false;
-}
-
 unsigned eights(long blocks) { return (unsigned)((blocks + 7) / 8 * 8); }
 
 template <typename T, int ACT>
@@ -1011,16 +1017,12 @@ int forward(int nhwc, const T* x, const wide_t<T>* gamma, const wide_t<T>* beta,
         GnLast g;
         auto whole = [&](int line, long most, auto threads, auto packs) {
             constexpr int N = decltype(threads)::value, M = decltype(packs)::value;
-            if (!whole_shape(&g, images, channels, pixels, groups, v, sizeof(T), line, N, M) || g.pieces > most ||
-                (g.pieces + 8) * N >= (1l << 32))
-                return false;
+            if (!whole_shape(&g, images, channels, pixels, groups, v, sizeof(T), line, most, N, M)) return false;
             hipLaunchKernelGGL((gn_last_whole<T, 16 / (int)sizeof(T), ACT, N, M>), dim3(eights(g.pieces)), dim3(N), 0, st, x,
                                gamma, beta, y, mean, inv_std, eps, g);
             return true;
         };
-        // packs of eight 16-bit values leave room for fewer threads
-        constexpr bool kShort = sizeof(T) == 2;
-        if (hold_slabs<4, 256, 16, kShort ? 512 : 1024, kShort ? 24 : 16>(whole)) {
+        if (hold_forward<sizeof(T) == 2>(whole)) {
             HIP_RETURN_IF_LAUNCH_FAILED();
             return PYDTNN_HIP_OK;
         }
@@ -1069,16 +1071,13 @@ int backward(int nhwc, const T* dy, const T* x, const wide_t<T>* gamma, const wi
         GnLast g;
         auto whole = [&](int line, long most, auto threads, auto packs) {
             constexpr int N = decltype(threads)::value, M = decltype(packs)::value;
-            if (!whole_shape(&g, images, channels, pixels, groups, v, sizeof(T), line, N, M) || g.pieces > most ||
-                (g.pieces + 8) * N >= (1l << 32))
-                return false;
+            if (!whole_shape(&g, images, channels, pixels, groups, v, sizeof(T), line, most, N, M)) return false;
             hipLaunchKernelGGL((gn_last_bwd_whole<T, 16 / (int)sizeof(T), ACT, N, M>), dim3(eights(g.pieces)), dim3(N), 0, st,
                                dy, x, gamma, beta, mean, inv_std, sums, dx, g);
             params(images);
             return true;
         };
-        constexpr bool kShort = sizeof(T) == 2;
-        if (hold_slabs<4, kShort ? 256 : 512, 8, kShort ? 512 : 1024, kShort ? 12 : 8>(whole)) {
+        if (hold_backward<sizeof(T) == 2>(whole)) {
             HIP_RETURN_IF_LAUNCH_FAILED();
             return PYDTNN_HIP_OK;
         }
@@ -1123,14 +1122,11 @@ int backward(int nhwc, const T* dy, const T* x, const wide_t<T>* gamma, const wi
 
 extern "C" {
 
-size_t pydtnn_hip_gn_workspace_bytes(int dtype, int nhwc, int backward, long images, long channels, long pixels, long groups)
+size_t pydtnn_hip_gn_workspace_bytes(int dtype, int nhwc, int backward, long images, long channels, long pixels, long groups,
+                                     int aligned)
 {
     if (check(images, channels, pixels, groups) != PYDTNN_HIP_OK || dtype < kDtypeF32 || dtype > kDtypeBF16) return 0;
-    const int c = (int)channels, p = (int)pixels, g = (int)groups;
-    const size_t a = workspace_of(pieces_of(dtype, nhwc, images, c, p, g, 1), images, g, backward != 0);
-    const size_t b = workspace_of(pieces_of(dtype, nhwc, images, c, p, g, pack_of(size_of(dtype), c, c / g)), images, g,
-                                  backward != 0);
-    return a > b ? a : b;
+    return workspace_bytes_of(dtype, nhwc != 0, backward != 0, images, (int)channels, (int)pixels, (int)groups, aligned != 0);
 }
 
 int pydtnn_hip_gn_forward(int dtype, int nhwc, const void* x, const void* gamma, const void* beta, void* y, void* mean,
@@ -1140,8 +1136,9 @@ int pydtnn_hip_gn_forward(int dtype, int nhwc, const void* x, const void* gamma,
     if (!x || !gamma || !beta || !y || !mean || !inv_std || !(eps >= 0.0)) return PYDTNN_HIP_ERR_INVALID;
     const int rc = check(images, channels, pixels, groups);
     if (rc != PYDTNN_HIP_OK) return rc;
-    if (!workspace || workspace_bytes < pydtnn_hip_gn_workspace_bytes(dtype, nhwc, 0, images, channels, pixels, groups))
-        return PYDTNN_HIP_ERR_WORKSPACE;
+    const size_t need = pydtnn_hip_gn_workspace_bytes(dtype, nhwc, 0, images, channels, pixels, groups,
+                                                      aligned16(x) && aligned16(y));
+    if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return PYDTNN_HIP_ERR_WORKSPACE;
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         using A = wide_t<T>;
@@ -1161,8 +1158,9 @@ int pydtnn_hip_gn_backward(int dtype, int nhwc, const void* dy, const void* x, c
     if (!dy || !x || !gamma || !beta || !mean || !inv_std || !dgamma || !dbeta) return PYDTNN_HIP_ERR_INVALID;
     const int rc = check(images, channels, pixels, groups);
     if (rc != PYDTNN_HIP_OK) return rc;
-    if (!workspace || workspace_bytes < pydtnn_hip_gn_workspace_bytes(dtype, nhwc, 1, images, channels, pixels, groups))
-        return PYDTNN_HIP_ERR_WORKSPACE;
+    const size_t need = pydtnn_hip_gn_workspace_bytes(dtype, nhwc, 1, images, channels, pixels, groups,
+                                                      aligned16(x) && aligned16(dy) && aligned16(dx));
+    if (!workspace || !aligned16(workspace) || workspace_bytes < need) return PYDTNN_HIP_ERR_WORKSPACE;
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         using A = wide_t<T>;

@@ -112,7 +112,7 @@ SIGNATURES = {
                                                             _vp]),
     "pydtnn_hip_bn_training_bwd_f64": (_c.c_int, [_vp] * 7 + [_c.c_long, _c.c_int, _c.c_long, _vp]),
     # several element types
-    "pydtnn_hip_gn_workspace_bytes": (_c.c_size_t, [_c.c_int] * 3 + [_c.c_long] * 4),
+    "pydtnn_hip_gn_workspace_bytes": (_c.c_size_t, [_c.c_int] * 3 + [_c.c_long] * 4 + [_c.c_int]),
     "pydtnn_hip_gn_forward": (_c.c_int, [_c.c_int, _c.c_int] + [_vp] * 6 + [_c.c_long] * 4 + [_c.c_double, _c.c_int, _vp,
                                                                                          _c.c_size_t, _vp]),
     "pydtnn_hip_gn_backward": (_c.c_int, [_c.c_int, _c.c_int] + [_vp] * 9 + [_c.c_long] * 4 + [_c.c_int, _vp, _c.c_size_t,
@@ -173,6 +173,27 @@ def ptr(t):
     if not t.is_contiguous():
         raise ValueError("expected a C-contiguous tensor")
     return ctypes.c_void_p(t.data_ptr())
+
+
+def address(t):
+    """``ptr`` as a plain number, which ctypes converts faster than an object."""
+    if t is None:
+        return None
+    if not t.is_cuda:
+        raise ValueError("expected a tensor on the GPU")
+    if not t.is_contiguous():
+        raise ValueError("expected a C-contiguous tensor")
+    return t.data_ptr()
+
+
+# The handle of a device's current stream without an object around it (0.1 instead of 2.7 us), where torch has the call.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def raw_stream(x):
+    """The current stream of the device of ``x``."""
+    return _raw_stream(x.device.index)
 
 
 def f32(t, name="tensor"):

@@ -10,7 +10,7 @@ import math
 import torch
 
 from . import native
-from .native import check, f32, lib, ptr, stream_ptr
+from .native import address, check, f32, lib, ptr, raw_stream, stream_ptr
 
 
 def _out_hw(h, w, kh, kw, vpadding, hpadding, vstride, hstride, vdilation, hdilation):
@@ -552,9 +552,9 @@ def _need_like(x, dtype, **tensors):
 
 
 def _scratch(nbytes, x):
-    """Scratch memory of one call.  It is the caller's alone: under capture it belongs to the graph that is captured, and
-    no other graph or later call is handed the same memory while this one can still run."""
-    return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=x.device)
+    """Scratch memory of one call, None for no bytes.  It is the call's alone: under capture it belongs to the graph that
+    is captured, and no other graph or later call is handed the same memory while this one can still run."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
 
 
 _GN_ACTIVATIONS = {"": 0, None: 0, "relu": 1, "silu": 2}
@@ -576,12 +576,16 @@ def _gn_extents(x, gamma, beta, groups, activation, nhwc):
     return x.shape[0], channels, pixels, groups, _GN_ACTIVATIONS[activation]
 
 
+def _is_aligned(*tensors):
+    return all(t.data_ptr() % 16 == 0 for t in tensors)
+
+
 @_on_its_device
 def gn_forward(x, gamma, beta, groups, eps=1e-5, activation="", nhwc=True):
     """Group normalisation with an activation (None, "relu" or "silu"): y = act(gamma * (x - mean) * inv_std + beta) with
     the statistics of each image's groups of consecutive channels, of shape (batch, groups).  ``x`` is (batch, ...,
-    channels), with ``nhwc=False`` (batch, channels, ...), in float32, float64, float16 or bfloat16; gamma, beta, mean and
-    inv_std are float32 (float64 for float64).  Returns (y, mean, inv_std)."""
+    channels), with ``nhwc=False`` (batch, channels, ...), in float32, float64, float16 or bfloat16; gamma, beta, mean
+    and inv_std are float32 (float64 for float64).  Returns (y, mean, inv_std)."""
     dtype = _dtype_of(x)
     images, channels, pixels, groups, act = _gn_extents(x, gamma, beta, groups, activation, nhwc)
     if not eps >= 0:
@@ -591,11 +595,12 @@ def gn_forward(x, gamma, beta, groups, eps=1e-5, activation="", nhwc=True):
     mean = torch.empty((images, groups), dtype=gamma.dtype, device=x.device)
     inv_std = torch.empty_like(mean)
     if images:
-        nbytes = lib().pydtnn_hip_gn_workspace_bytes(dtype, int(nhwc), 0, images, channels, pixels, groups)
+        nbytes = lib().pydtnn_hip_gn_workspace_bytes(dtype, int(nhwc), 0, images, channels, pixels, groups,
+                                                     _is_aligned(x, y))
         ws = _scratch(nbytes, x)
-        check(lib().pydtnn_hip_gn_forward(dtype, int(nhwc), ptr(x), ptr(gamma), ptr(beta), ptr(y), ptr(mean), ptr(inv_std),
-                                          images, channels, pixels, groups, float(eps), act, ptr(ws), nbytes, stream_ptr()),
-              "gn_forward")
+        check(lib().pydtnn_hip_gn_forward(dtype, int(nhwc), address(x), address(gamma), address(beta), address(y),
+                                          address(mean), address(inv_std), images, channels, pixels, groups, float(eps),
+                                          act, address(ws), nbytes, raw_stream(x)), "gn_forward")
     return y, mean, inv_std
 
 
@@ -611,20 +616,23 @@ def gn_backward(dy, x, gamma, beta, mean, inv_std, groups, activation="", nhwc=T
     dx = torch.empty_like(x) if need_dx else None
     if not images:
         return dgamma.zero_(), dbeta.zero_(), dx
-    nbytes = lib().pydtnn_hip_gn_workspace_bytes(dtype, int(nhwc), 1, images, channels, pixels, groups)
+    # (a dx that is not asked for is as good as aligned)
+    nbytes = lib().pydtnn_hip_gn_workspace_bytes(dtype, int(nhwc), 1, images, channels, pixels, groups,
+                                                 _is_aligned(x, dy))
     ws = _scratch(nbytes, x)
-    check(lib().pydtnn_hip_gn_backward(dtype, int(nhwc), ptr(dy), ptr(x), ptr(gamma), ptr(beta), ptr(mean), ptr(inv_std),
-                                       ptr(dgamma), ptr(dbeta), ptr(dx), images, channels, pixels, groups, act, ptr(ws),
-                                       nbytes, stream_ptr()), "gn_backward")
+    check(lib().pydtnn_hip_gn_backward(dtype, int(nhwc), address(dy), address(x), address(gamma), address(beta),
+                                       address(mean), address(inv_std), address(dgamma), address(dbeta), address(dx),
+                                       images, channels, pixels, groups, act, address(ws), nbytes, raw_stream(x)),
+          "gn_backward")
     return dgamma, dbeta, dx
 
 
 @_on_its_device
 def dropout(x, rate, seed, offset=0):
     """``x`` with each element dropped (set to 0) with probability ``rate``, in steps of 2^-16, and the others divided by
-    the probability that they are kept.  The mask is a function of ``seed``, ``offset`` (64 bits each) and the element's index
-    alone and is stored nowhere: ``dropout_backward`` with the same numbers draws it again.  ``offset`` may be an int64
-    tensor of one element on the GPU: then a captured graph draws another mask whenever that number has changed."""
+    the probability that they are kept.  The mask is a function of ``seed``, ``offset`` (64 bits each) and the element's
+    index alone and is stored nowhere: ``dropout_backward`` with the same numbers draws it again.  ``offset`` may be an
+    int64 tensor of one element on the GPU: then a captured graph draws another mask whenever that number has changed."""
     dtype = _dtype_of(x)
     if not 0 <= rate <= 1:
         raise ValueError(f"the rate of dropout is {rate}, it has to be between 0 and 1")
@@ -634,13 +642,13 @@ def dropout(x, rate, seed, offset=0):
             raise TypeError("the offset of dropout is a number or an int64 tensor of one element")
         if offset.device != x.device:
             raise ValueError(f"the offset is on {offset.device}, the tensor on {x.device}")
-        offset, offset_dev = 0, ptr(offset)
+        offset, offset_dev = 0, address(offset)
     x = x.contiguous()
     y = torch.empty_like(x)
     if x.numel():
         mask = (1 << 64) - 1
-        check(lib().pydtnn_hip_dropout(dtype, ptr(x), ptr(y), x.numel(), float(rate), int(seed) & mask, int(offset) & mask,
-                                       offset_dev, stream_ptr()), "dropout")
+        check(lib().pydtnn_hip_dropout(dtype, address(x), address(y), x.numel(), float(rate), int(seed) & mask,
+                                       int(offset) & mask, offset_dev, raw_stream(x)), "dropout")
     return y
 
 
@@ -667,25 +675,25 @@ def _need_fp8_input(x):
 @_on_its_device
 def quantize_fp8(x):
     """A (rows, k) matrix in e4m3 with a scale for each block of 128 consecutive elements of a row -> (q, scales).  q is
-    (rows, k to a multiple of 128), zeros behind k; scales holds e + 127 for the scale 2^e of a block, the smallest that brings
-    the block within 448, the largest e4m3 value (rows, blocks to a multiple of 4, uint8).  A block with an infinity or a NaN
-    becomes NaN throughout."""
+    (rows, k to a multiple of 128), zeros behind k; scales holds e + 127 for the scale 2^e of a block, the smallest that
+    brings the block within 448, the largest e4m3 value (rows, blocks to a multiple of 4, uint8).  A block with an
+    infinity or a NaN becomes NaN throughout."""
     dtype = _need_fp8_input(x)
     x = x.contiguous()
     q_shape, scales_shape = _fp8_shapes(*x.shape)
     q = torch.empty(q_shape, dtype=torch.float8_e4m3fn, device=x.device)
     scales = torch.empty(scales_shape, dtype=torch.uint8, device=x.device)
     if x.shape[0]:
-        check(lib().pydtnn_hip_quantize_fp8(dtype, ptr(x), x.shape[0], x.shape[1], ptr(q), ptr(scales), stream_ptr()),
-              "quantize_fp8")
+        check(lib().pydtnn_hip_quantize_fp8(dtype, address(x), x.shape[0], x.shape[1], address(q), address(scales),
+                                            raw_stream(x)), "quantize_fp8")
     return q, scales
 
 
 @_on_its_device
 def matmul_fp8(x, wq, wscales, bias=None, relu=False):
     """``x @ w.T (+ bias, ReLU)`` in e4m3 for (m, k) activations, which are quantised on the way, and weights that
-    ``quantize_fp8`` has made of an (n, k) matrix once.  Sums are held in 32 bits, bias is float32, the result has the type of
-    ``x``."""
+    ``quantize_fp8`` has made of an (n, k) matrix once.  Sums are held in 32 bits, bias is float32, the result has the
+    type of ``x``."""
     dtype = _need_fp8_input(x)
     m, k = x.shape
     if wq.dim() != 2 or wq.shape[0] < 1:
@@ -701,6 +709,6 @@ def matmul_fp8(x, wq, wscales, bias=None, relu=False):
     if m:
         nbytes = lib().pydtnn_hip_matmul_fp8_workspace_bytes(dtype, m, n, k)
         ws = _scratch(nbytes, x)
-        check(lib().pydtnn_hip_matmul_fp8(dtype, ptr(x), m, k, ptr(wq), ptr(wscales), n, ptr(bias), int(relu), ptr(y), ptr(ws),
-                                          nbytes, stream_ptr()), "matmul_fp8")
+        check(lib().pydtnn_hip_matmul_fp8(dtype, address(x), m, k, address(wq), address(wscales), n, address(bias),
+                                          int(relu), address(y), address(ws), nbytes, raw_stream(x)), "matmul_fp8")
     return y

@@ -67,8 +67,8 @@ def test_gn_refuses_extents_it_cannot_run(lib):
     p = ctypes.c_void_p(FAKE)
 
     def forward(dtype=0, images=2, channels=8, pixels=4, groups=2, eps=1e-5, act=0, x=p, nbytes=None):
-        need = lib.pydtnn_hip_gn_workspace_bytes(dtype, 1, 0, images, channels, pixels, groups)
-        return lib.pydtnn_hip_gn_forward(dtype, 1, x, p, p, p, p, p, images, channels, pixels, groups, eps, act, p,
+        need = lib.pydtnn_hip_gn_workspace_bytes(dtype, 0, 0, images, channels, pixels, groups, 1)
+        return lib.pydtnn_hip_gn_forward(dtype, 0, x, p, p, p, p, p, images, channels, pixels, groups, eps, act, p,
                                          need - 1 if nbytes else need, None)
 
     assert forward(x=None) == 1
@@ -171,7 +171,9 @@ def test_fp8_refuses_what_it_cannot_run(lib):
     assert matmul(x=None) == matmul(w=None) == matmul(s=None) == matmul(y=None) == 1
     assert matmul(m=0) == matmul(k=0) == matmul(n=0) == matmul(dtype=1) == 1
     assert matmul(w=ctypes.c_void_p(FAKE + 8)) == 1
-    assert matmul(ws=None) == matmul(short=1) == matmul(ws=ctypes.c_void_p(FAKE + 4)) == 2
+    # (a few short rows need no workspace)
+    assert lib.pydtnn_hip_matmul_fp8_workspace_bytes(0, 4, 6, 200) == 0
+    assert matmul(m=40, ws=None) == matmul(m=40, short=1) == matmul(m=40, ws=ctypes.c_void_p(FAKE + 4)) == 2
     assert matmul(n=(1 << 30) + 1) == 4
 
 
