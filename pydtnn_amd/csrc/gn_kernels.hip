@@ -42,14 +42,6 @@ __device__ __forceinline__ A act(A z)
     return z;
 }
 
-template <typename A>
-__device__ __forceinline__ A wave_sum(A v)
-{
-#pragma unroll
-    for (int o = kWave / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
-    return v;
-}
-
 // The sum over `lanes` consecutive lanes, a power of two, in each of them.
 template <typename A>
 __device__ __forceinline__ A lanes_sum(A v, int lanes)
@@ -160,7 +152,10 @@ __device__ __forceinline__ void each_pixel_of_two(const Place& at, int rows, con
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) f(v[u], w[u], p + u * rows);
     }
-    for (; p < at.p1; p += rows) f(x[p * step], y[p * step], p);
+    for (; p < at.p1; p += rows) {
+        P v = x[p * step], w = y[p * step];
+        f(v, w, p);
+    }
 }
 
 // Moments of one thread's elements of each of V channels, from differences from its own first element.
@@ -458,8 +453,9 @@ struct ChansBwd {
         }
     }
 
-    template <int ACT, typename T>
-    __device__ __forceinline__ void add(const Pack<T, V>& x, const Pack<T, V>& dy, A* s1, A* s2) const
+    // With KEEP, dz takes the place of dy: for apply<kIdentity> later.
+    template <int ACT, bool KEEP, typename T>
+    __device__ __forceinline__ void add(const Pack<T, V>& x, Pack<T, V>& dy, A* s1, A* s2) const
     {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -467,6 +463,7 @@ struct ChansBwd {
             const A dz = dz_of<ACT>(ch[j], (A)x.v[j], xn, (A)dy.v[j]);
             s1[j] += dz;
             s2[j] += dz * xn;
+            if (KEEP) dy.v[j] = (T)dz;
         }
     }
 
@@ -531,7 +528,7 @@ __global__ void __launch_bounds__(kT) gn_last_bwd_sums(const T* __restrict__ dy,
             ch.template set<ACT>(g, at.image, at.slab * g.width + c, mean, inv_std, gamma, beta);
             each_pixel_of_two(at, g.rows, reinterpret_cast<const Pack<T, V>*>(x + base + c),
                               reinterpret_cast<const Pack<T, V>*>(dy + base + c), g.channels / V,
-                              [&](const Pack<T, V>& xv, const Pack<T, V>& dv, int) { ch.template add<ACT>(xv, dv, s1, s2); });
+                              [&](const Pack<T, V>& xv, Pack<T, V>& dv, int) { ch.template add<ACT, false>(xv, dv, s1, s2); });
         }
         join_rows<kT, V>(g, c0, s1, s2, [&](int i, A t1, A t2) {
             out1[i] = t1;
@@ -677,12 +674,14 @@ __global__ void __launch_bounds__(THREADS) gn_last_bwd_whole(const T* __restrict
             dv[i] = din[(at.ty + i * g.rows) * step];
         }
     }
+    // dz is computed once where its type holds it: of the rectifier it is dy or 0
+    constexpr bool kKeep = ACT != kSilu || sizeof(T) >= 4;
     ChansBwd<A, V> ch;
     A s1[V] = {}, s2[V] = {};
     if (mine) ch.template set<ACT>(g, at.image, at.slab * g.width + at.tx * V, mean, inv_std, gamma, beta);
 #pragma unroll
     for (int i = 0; i < PACKS; ++i)
-        if (i < mine) ch.template add<ACT>(xv[i], dv[i], s1, s2);
+        if (i < mine) ch.template add<ACT, kKeep>(xv[i], dv[i], s1, s2);
     A* out1 = sums + at.image * g.channels + at.slab * g.width;
     A* out2 = out1 + g.images * g.channels;
     join_rows<THREADS, V>(g, 0, s1, s2, [&](int i, A t1, A t2) {
@@ -704,16 +703,55 @@ __global__ void __launch_bounds__(THREADS) gn_last_bwd_whole(const T* __restrict
     }
 #pragma unroll
     for (int i = 0; i < PACKS; ++i)
-        if (i < mine) out[(at.ty + i * g.rows) * step] = ch.template apply<ACT>(xv[i], dv[i], a, b);
+        if (i < mine) out[(at.ty + i * g.rows) * step] = ch.template apply<kKeep ? kIdentity : ACT>(xv[i], dv[i], a, b);
 }
 
 // ---------------------------------------------------------------------------------------------- channels first
-// A wave, or a workgroup where planes are large, takes a plane: one channel of one image.
-template <typename T, int THREADS>
-__device__ __forceinline__ wide_t<T> plane_sum(wide_t<T> v, wide_t<T>* part)
+// A group is one run of memory here.  Where a workgroup's registers hold it, one kernel does the forward pass; otherwise, and
+// in the backward pass, whose sums are of channels, THREADS threads take a plane: one channel of one image.
+struct GnFirst {
+    long planes;                     // images * channels
+    int pixels, channels, cg;
+    FastDiv by_pixels;               // exact for the elements of a group that one kernel holds, at most 2^16
+};
+
+// Calls f(pack of x, its number) for the packs of a plane, kAhead loads under way at once.
+template <int THREADS, typename P, typename F>
+__device__ __forceinline__ void each_pack(const P* x, int packs, F f)
 {
-    v = wave_sum(v);
-    if (THREADS == kWave) return v;
+    int p = threadIdx.x % THREADS;
+    for (; p + (kAhead - 1) * THREADS < packs; p += kAhead * THREADS) {
+        P v[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) v[u] = x[p + u * THREADS];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) f(v[u], p + u * THREADS);
+    }
+    for (; p < packs; p += THREADS) f(x[p], p);
+}
+
+template <int THREADS, typename P, typename F>
+__device__ __forceinline__ void each_pack_of_two(const P* x, const P* y, int packs, F f)
+{
+    int p = threadIdx.x % THREADS;
+    for (; p + (kAhead - 1) * THREADS < packs; p += kAhead * THREADS) {
+        P v[kAhead], w[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            v[u] = x[p + u * THREADS];
+            w[u] = y[p + u * THREADS];
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) f(v[u], w[u], p + u * THREADS);
+    }
+    for (; p < packs; p += THREADS) f(x[p], y[p], p);
+}
+
+template <int THREADS, typename A>
+__device__ __forceinline__ A plane_sum(A v, A* part)
+{
+    v = lanes_sum(v, THREADS < kWave ? THREADS : kWave);
+    if (THREADS <= kWave) return v;
     __syncthreads();
     if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = v;
     __syncthreads();
@@ -723,106 +761,184 @@ __device__ __forceinline__ wide_t<T> plane_sum(wide_t<T> v, wide_t<T>* part)
     return v;
 }
 
-template <typename T, int THREADS>
+template <int THREADS>
+__device__ __forceinline__ long plane_of()
+{
+    return (long)blockIdx.x * (kT / THREADS) + threadIdx.x / THREADS;
+}
+
+template <typename T, int V, int THREADS>
 __global__ void __launch_bounds__(kT) gn_first_moments(const T* __restrict__ x, Moments<wide_t<T>>* __restrict__ partial,
-                                                       long planes, int pixels)
+                                                       GnFirst g)
 {
     using A = wide_t<T>;
     __shared__ A part[kWaves];
-    const long plane = (long)blockIdx.x * (kT / THREADS) + threadIdx.x / THREADS;
-    if (plane >= planes) return;
-    const T* base = x + plane * pixels;
+    const long plane = plane_of<THREADS>();
+    if (plane >= g.planes) return;
+    const T* base = x + plane * g.pixels;
+    const Pack<T, V>* packs = reinterpret_cast<const Pack<T, V>*>(base);
     const A first = (A)base[0];
     A s1 = (A)0;
-    for (int p = threadIdx.x % THREADS; p < pixels; p += THREADS) s1 += (A)base[p] - first;
-    const A mean = first + plane_sum<T, THREADS>(s1, part) / (A)pixels;
+    each_pack<THREADS>(packs, g.pixels / V, [&](const Pack<T, V>& v, int) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) s1 += (A)v.v[j] - first;
+    });
+    const A mean = first + plane_sum<THREADS>(s1, part) / (A)g.pixels;
     A s2 = (A)0;
-    for (int p = threadIdx.x % THREADS; p < pixels; p += THREADS) {
-        const A d = (A)base[p] - mean;
-        s2 += d * d;
-    }
-    s2 = plane_sum<T, THREADS>(s2, part);
+    each_pack<THREADS>(packs, g.pixels / V, [&](const Pack<T, V>& v, int) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) s2 += ((A)v.v[j] - mean) * ((A)v.v[j] - mean);
+    });
+    s2 = plane_sum<THREADS>(s2, part);
     if (threadIdx.x % THREADS == 0) partial[plane] = Moments<A>{mean, s2};
 }
 
-template <typename T, int THREADS, int ACT>
+template <typename T, int V, int THREADS, int ACT>
 __global__ void __launch_bounds__(kT) gn_first_apply(const T* __restrict__ x, const wide_t<T>* __restrict__ gamma,
                                                      const wide_t<T>* __restrict__ beta,
                                                      const Moments<wide_t<T>>* __restrict__ partial, T* __restrict__ y,
                                                      wide_t<T>* __restrict__ mean_out, wide_t<T>* __restrict__ inv_std_out,
-                                                     double eps, long planes, int pixels, int channels, int cg)
+                                                     double eps, GnFirst g)
 {
     using A = wide_t<T>;
-    const long plane = (long)blockIdx.x * (kT / THREADS) + threadIdx.x / THREADS;
-    if (plane >= planes) return;
-    const long group = plane / cg;
-    const int c = (int)(plane % channels);
+    const long plane = plane_of<THREADS>();
+    if (plane >= g.planes) return;
+    const long group = plane / g.cg;
+    const int c = (int)(plane % g.channels);
     A mean, inv_std;
-    join_moments<A>(partial + group * cg, cg, [&](int) { return (double)pixels; }, (double)pixels * cg, eps, kWave, &mean,
-                    &inv_std);
-    if (plane % cg == 0 && threadIdx.x % THREADS == 0) {
+    join_moments<A>(partial + group * g.cg, g.cg, [&](int) { return (double)g.pixels; }, (double)g.pixels * g.cg, eps,
+                    THREADS < kWave ? THREADS : kWave, &mean, &inv_std);
+    if (plane % g.cg == 0 && threadIdx.x % THREADS == 0) {
         mean_out[group] = mean;
         inv_std_out[group] = inv_std;
     }
     const A scale = inv_std * gamma[c], shift = beta[c];
-    for (int p = threadIdx.x % THREADS; p < pixels; p += THREADS) {
-        const long i = plane * pixels + p;
-        y[i] = (T)act<ACT>(((A)x[i] - mean) * scale + shift);
+    Pack<T, V>* out = reinterpret_cast<Pack<T, V>*>(y + plane * g.pixels);
+    each_pack<THREADS>(reinterpret_cast<const Pack<T, V>*>(x + plane * g.pixels), g.pixels / V,
+                       [&](Pack<T, V> v, int p) {
+#pragma unroll
+                           for (int j = 0; j < V; ++j) v.v[j] = (T)act<ACT>(((A)v.v[j] - mean) * scale + shift);
+                           stream_out(out + p, v);
+                       });
+}
+
+// A workgroup holds a group: x is read once.  `join` makes one group of all threads for join_threads.
+template <typename T, int V, int ACT, int THREADS, int PACKS>
+__global__ void __launch_bounds__(THREADS) gn_first_whole(const T* __restrict__ x, const wide_t<T>* __restrict__ gamma,
+                                                          const wide_t<T>* __restrict__ beta, T* __restrict__ y,
+                                                          wide_t<T>* __restrict__ mean_out,
+                                                          wide_t<T>* __restrict__ inv_std_out, double eps, GnFirst g, GnLast join)
+{
+    using A = wide_t<T>;
+    __shared__ A mean, inv_std;
+    const long group = blockIdx.x, elements = (long)g.cg * g.pixels;
+    const int c0 = (int)(group % (g.channels / g.cg)) * g.cg, packs = (int)(elements / V);
+    const Pack<T, V>* in = reinterpret_cast<const Pack<T, V>*>(x + group * elements);
+    Pack<T, V>* out = reinterpret_cast<Pack<T, V>*>(y + group * elements);
+    Pack<T, V> v[PACKS];
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i)
+        if ((int)threadIdx.x + i * THREADS < packs) v[i] = in[threadIdx.x + i * THREADS];
+    ThreadMoments<A, 1> t = {};      // all of one group
+    if ((int)threadIdx.x < packs) t.first[0] = (A)v[0].v[0];
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i) {
+        if ((int)threadIdx.x + i * THREADS >= packs) continue;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const A d = (A)v[i].v[j] - t.first[0];
+            t.s1[0] += d;
+            t.s2[0] += d * d;
+        }
+        t.n += V;
+    }
+    join_threads<THREADS>(join, t, [&](int, double count, double m, double m2) {
+        mean_out[group] = mean = (A)m;
+        inv_std_out[group] = inv_std = (A)(1.0 / sqrt(m2 / count + eps));
+    });
+    __syncthreads();
+    const A mu = mean, r = inv_std;
+    const bool one = g.pixels % V == 0;      // whether a pack is of one channel
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i) {
+        const int p = threadIdx.x + i * THREADS;
+        if (p >= packs) continue;
+        int c = c0 + (int)fd_div((uint32_t)(p * V), g.by_pixels);
+        A scale = r * gamma[c], shift = beta[c];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if (!one && j > 0) {
+                c = c0 + (int)fd_div((uint32_t)(p * V + j), g.by_pixels);
+                scale = r * gamma[c];
+                shift = beta[c];
+            }
+            v[i].v[j] = (T)act<ACT>(((A)v[i].v[j] - mu) * scale + shift);
+        }
+        out[p] = v[i];
     }
 }
 
-template <typename T, int THREADS, int ACT>
+template <typename T, int V, int THREADS, int ACT>
 __global__ void __launch_bounds__(kT) gn_first_bwd_sums(const T* __restrict__ dy, const T* __restrict__ x,
                                                         const wide_t<T>* __restrict__ gamma,
                                                         const wide_t<T>* __restrict__ beta,
                                                         const wide_t<T>* __restrict__ mean,
                                                         const wide_t<T>* __restrict__ inv_std,
-                                                        wide_t<T>* __restrict__ sums, long planes, int pixels, int channels,
-                                                        int cg)
+                                                        wide_t<T>* __restrict__ sums, GnFirst g)
 {
     using A = wide_t<T>;
     __shared__ A part[kWaves];
-    const long plane = (long)blockIdx.x * (kT / THREADS) + threadIdx.x / THREADS;
-    if (plane >= planes) return;
-    const int c = (int)(plane % channels);
-    const ChanBwd<A> ch = chan_bwd<ACT>(mean[plane / cg], inv_std[plane / cg], gamma[c], beta[c]);
+    const long plane = plane_of<THREADS>();
+    if (plane >= g.planes) return;
+    const int c = (int)(plane % g.channels);
+    const ChanBwd<A> ch = chan_bwd<ACT>(mean[plane / g.cg], inv_std[plane / g.cg], gamma[c], beta[c]);
     A s1 = (A)0, s2 = (A)0;
-    for (int p = threadIdx.x % THREADS; p < pixels; p += THREADS) {
-        const long i = plane * pixels + p;
-        const A xn = ((A)x[i] - ch.mean) * ch.inv_std;
-        const A dz = dz_of<ACT>(ch, (A)x[i], xn, (A)dy[i]);
-        s1 += dz;
-        s2 += dz * xn;
-    }
-    s1 = plane_sum<T, THREADS>(s1, part);
-    s2 = plane_sum<T, THREADS>(s2, part);
+    each_pack_of_two<THREADS>(reinterpret_cast<const Pack<T, V>*>(x + plane * g.pixels),
+                              reinterpret_cast<const Pack<T, V>*>(dy + plane * g.pixels), g.pixels / V,
+                              [&](const Pack<T, V>& xv, const Pack<T, V>& dv, int) {
+#pragma unroll
+                                  for (int j = 0; j < V; ++j) {
+                                      const A xn = ((A)xv.v[j] - ch.mean) * ch.inv_std;
+                                      const A dz = dz_of<ACT>(ch, (A)xv.v[j], xn, (A)dv.v[j]);
+                                      s1 += dz;
+                                      s2 += dz * xn;
+                                  }
+                              });
+    s1 = plane_sum<THREADS>(s1, part);
+    s2 = plane_sum<THREADS>(s2, part);
     if (threadIdx.x % THREADS == 0) {
         sums[plane] = s1;
-        sums[planes + plane] = s2;
+        sums[g.planes + plane] = s2;
     }
 }
 
-template <typename T, int THREADS, int ACT>
+template <typename T, int V, int THREADS, int ACT>
 __global__ void __launch_bounds__(kT) gn_first_bwd_apply(const T* __restrict__ dy, const T* __restrict__ x,
                                                          const wide_t<T>* __restrict__ gamma,
                                                          const wide_t<T>* __restrict__ beta,
                                                          const wide_t<T>* __restrict__ mean,
                                                          const wide_t<T>* __restrict__ inv_std,
-                                                         const wide_t<T>* __restrict__ ab, T* __restrict__ dx, long planes,
-                                                         int pixels, int channels, int cg)
+                                                         const wide_t<T>* __restrict__ ab, T* __restrict__ dx, GnFirst g)
 {
     using A = wide_t<T>;
-    const long plane = (long)blockIdx.x * (kT / THREADS) + threadIdx.x / THREADS;
-    if (plane >= planes) return;
-    const int c = (int)(plane % channels);
-    const long group = plane / cg;
+    const long plane = plane_of<THREADS>();
+    if (plane >= g.planes) return;
+    const int c = (int)(plane % g.channels);
+    const long group = plane / g.cg;
     const ChanBwd<A> ch = chan_bwd<ACT>(mean[group], inv_std[group], gamma[c], beta[c]);
     const A a = ab[2 * group], b = ab[2 * group + 1];
-    for (int p = threadIdx.x % THREADS; p < pixels; p += THREADS) {
-        const long i = plane * pixels + p;
-        const A xn = ((A)x[i] - ch.mean) * ch.inv_std;
-        dx[i] = (T)dx_of(ch, xn, dz_of<ACT>(ch, (A)x[i], xn, (A)dy[i]), a, b);
-    }
+    Pack<T, V>* out = reinterpret_cast<Pack<T, V>*>(dx + plane * g.pixels);
+    each_pack_of_two<THREADS>(reinterpret_cast<const Pack<T, V>*>(x + plane * g.pixels),
+                              reinterpret_cast<const Pack<T, V>*>(dy + plane * g.pixels), g.pixels / V,
+                              [&](const Pack<T, V>& xv, Pack<T, V> dv, int p) {
+#pragma unroll
+                                  for (int j = 0; j < V; ++j) {
+                                      const A xn = ((A)xv.v[j] - ch.mean) * ch.inv_std;
+                                      const A dz = dz_of<ACT>(ch, (A)xv.v[j], xn, (A)dv.v[j]);
+                                      dv.v[j] = (T)dx_of(ch, xn, dz, a, b);
+                                  }
+                                  stream_out(out + p, dv);
+                              });
 }
 
 // A and B of each group: one wave a group.
@@ -928,8 +1044,9 @@ int check(long images, long channels, long pixels, long groups)
 
 int size_of(int dtype) { return dtype == kDtypeF64 ? 8 : dtype == kDtypeF32 ? 4 : 2; }
 
-// Calls launch(line, most, threads, packs) for the ways to hold a slab, the better first, until one fits: 256 threads before more
-// (several workgroups to a compute unit, whose loads and stores overlap) and whole lines of 128 bytes before half lines
+// Calls launch(line, most, threads, packs) for the ways to hold a slab, the better first, until one fits: few threads before
+// many (several workgroups to a compute unit, whose loads and stores overlap), eight packs to a thread rather than sixteen
+// (forward 16 x 28 x 28 x 512 in bfloat16: 12 us and 15) and whole lines of 128 bytes before half lines
 // (forward 64 x 14 x 14 x 1024 in float32: 19 us with lines, 22 with half lines).  The largest workgroup has a compute unit
 // to itself and is taken where one round of them does it all: forward 56 x 56 x 256 in float32 takes 22 us against 30 in two
 // passes for 16 images (256 slabs), 103 against 102 for 64.
@@ -950,13 +1067,37 @@ bool hold_slabs(F launch)
 template <bool SHORT, typename F>
 bool hold_forward(F launch)
 {
-    return hold_slabs<4, 256, 16, SHORT ? 512 : 1024, SHORT ? 24 : 16>(launch);
+    return hold_slabs<4, 512, 8, SHORT ? 512 : 1024, SHORT ? 24 : 16>(launch);
 }
 
 template <bool SHORT, typename F>
 bool hold_backward(F launch)
 {
     return hold_slabs<4, SHORT ? 256 : 512, 8, SHORT ? 512 : 1024, SHORT ? 12 : 8>(launch);
+}
+
+// Calls launch(threads, packs) for the smallest workgroup whose registers hold `packs` packs of a group that is one run of
+// memory; whether there is one.  SHORT: packs of eight 16-bit values, of which a thread holds fewer (64 x 256 x 56 x 56 in
+// bfloat16: 55 us with eight each to 512 threads, 72 with sixteen to 256; in float32 89 with sixteen to 512, 106 with eight to
+// 1024).
+template <bool SHORT, typename F>
+bool hold_group(long packs, F launch)
+{
+    using std::integral_constant;
+    if (packs <= 256 * 4) launch(integral_constant<int, 256>(), integral_constant<int, 4>());
+    else if (packs <= 512 * 8) launch(integral_constant<int, 512>(), integral_constant<int, 8>());
+    else if (packs <= 1024 * 8) launch(integral_constant<int, SHORT ? 1024 : 512>(), integral_constant<int, SHORT ? 8 : 16>());
+    else if (packs <= 1024 * 16 && !SHORT) launch(integral_constant<int, 1024>(), integral_constant<int, SHORT ? 8 : 16>());
+    else return false;
+    return true;
+}
+
+bool first_whole(int size, int pixels, int cg, bool aligned, long groups)
+{
+    const long elements = (long)cg * pixels;
+    auto any = [](auto, auto) {};
+    return aligned && elements % (16 / size) == 0 && groups * 1024 < (1l << 32) &&
+           (size == 2 ? hold_group<true>(elements * size / 16, any) : hold_group<false>(elements * size / 16, any));
 }
 
 size_t workspace_bytes_of(int dtype, bool nhwc, bool backward, long images, int channels, int pixels, int groups, bool aligned)
@@ -973,6 +1114,8 @@ size_t workspace_bytes_of(int dtype, bool nhwc, bool backward, long images, int 
         const GnLast g = last_shape(images, channels, pixels, groups, v);
         moments = images * groups * g.splits;
         sums = images * channels * g.splits;
+    } else if (!backward && first_whole(size, pixels, channels / groups, aligned, images * groups)) {
+        return 0;
     }
     return (size_t)(backward ? 2 * sums + 2 * images * groups : 2 * moments) * wide;
 }
@@ -1001,8 +1144,24 @@ int with_pack(int v, F f)
 
 bool too_many(long blocks) { return blocks * kT >= (1l << 32); }      // a launch counts its threads in 32 bits
 
-// Planes of fewer pixels than this go to a wave each.
-constexpr int kPlaneOfGroup = 1024;
+// Calls launch(elements of a pack, threads of a plane) for channels first: eight packs or more to a thread, where a plane has
+// them, so that small planes share workgroups.
+template <typename T, typename F>
+int with_plane(int pixels, bool aligned, F launch)
+{
+    using std::integral_constant;
+    constexpr int V = 16 / sizeof(T);
+    auto threads = [&](auto v) {
+        const int packs = pixels / decltype(v)::value;
+        if (packs < 16 * 8) return launch(v, integral_constant<int, 16>());
+        if (packs < kWave * 8) return launch(v, integral_constant<int, kWave>());
+        return launch(v, integral_constant<int, kT>());
+    };
+    if (aligned && pixels % V == 0) return threads(integral_constant<int, V>());
+    return threads(integral_constant<int, 1>());
+}
+
+long plane_blocks(long planes, int threads) { return (planes + kT / threads - 1) / (kT / threads); }
 
 unsigned eights(long blocks) { return (unsigned)((blocks + 7) / 8 * 8); }
 
@@ -1037,20 +1196,31 @@ int forward(int nhwc, const T* x, const wide_t<T>* gamma, const wide_t<T>* beta,
             return PYDTNN_HIP_OK;
         });
     }
-    const long planes = images * channels;
-    const bool small = pixels < kPlaneOfGroup;
-    const long blocks = small ? (planes + kWaves - 1) / kWaves : planes;
-    if (too_many(blocks)) return PYDTNN_HIP_ERR_UNSUPPORTED;
-    auto launch = [&](auto threads) {
-        constexpr int N = decltype(threads)::value;
-        hipLaunchKernelGGL((gn_first_moments<T, N>), dim3((unsigned)blocks), dim3(kT), 0, st, x, part, planes, pixels);
-        hipLaunchKernelGGL((gn_first_apply<T, N, ACT>), dim3((unsigned)blocks), dim3(kT), 0, st, x, gamma, beta, part, y,
-                           mean, inv_std, eps, planes, pixels, channels, channels / groups);
-    };
-    if (small) launch(std::integral_constant<int, kWave>());
-    else launch(std::integral_constant<int, kT>());
-    HIP_RETURN_IF_LAUNCH_FAILED();
-    return PYDTNN_HIP_OK;
+    const int cg = channels / groups;
+    const GnFirst g = {images * channels, pixels, channels, cg, make_fastdiv((uint32_t)pixels)};
+    const bool aligned = aligned16(x) && aligned16(y);
+    if (first_whole(sizeof(T), pixels, cg, aligned, images * groups)) {
+        constexpr int V = 16 / sizeof(T);
+        hold_group<sizeof(T) == 2>((long)cg * pixels / V, [&](auto threads, auto packs) {
+            constexpr int N = decltype(threads)::value, M = decltype(packs)::value;
+            GnLast join = {images, pixels, 1, 1, 1, 1, 1, 1, N, 1, 1, 1, 1, 1, 1, {}};
+            set_joins(&join, N, 1);
+            hipLaunchKernelGGL((gn_first_whole<T, V, ACT, N, M>), dim3((unsigned)(images * groups)), dim3(N), 0, st, x, gamma,
+                               beta, y, mean, inv_std, eps, g, join);
+        });
+        HIP_RETURN_IF_LAUNCH_FAILED();
+        return PYDTNN_HIP_OK;
+    }
+    return with_plane<T>(pixels, aligned, [&](auto pack, auto threads) {
+        constexpr int V = decltype(pack)::value, N = decltype(threads)::value;
+        const long blocks = plane_blocks(g.planes, N);
+        if (too_many(blocks)) return PYDTNN_HIP_ERR_UNSUPPORTED;
+        hipLaunchKernelGGL((gn_first_moments<T, V, N>), dim3((unsigned)blocks), dim3(kT), 0, st, x, part, g);
+        hipLaunchKernelGGL((gn_first_apply<T, V, N, ACT>), dim3((unsigned)blocks), dim3(kT), 0, st, x, gamma, beta, part, y,
+                           mean, inv_std, eps, g);
+        HIP_RETURN_IF_LAUNCH_FAILED();
+        return PYDTNN_HIP_OK;
+    });
 }
 
 template <typename T, int ACT>
@@ -1096,26 +1266,24 @@ int backward(int nhwc, const T* dy, const T* x, const wide_t<T>* gamma, const wi
             return PYDTNN_HIP_OK;
         });
     }
-    const long planes = images * channels;
-    const bool small = pixels < kPlaneOfGroup;
-    const long blocks = small ? (planes + kWaves - 1) / kWaves : planes;
-    if (too_many(blocks)) return PYDTNN_HIP_ERR_UNSUPPORTED;
-    auto launch = [&](auto threads) {
-        constexpr int N = decltype(threads)::value;
-        A* ab = sums + 2 * planes;
-        hipLaunchKernelGGL((gn_first_bwd_sums<T, N, ACT>), dim3((unsigned)blocks), dim3(kT), 0, st, dy, x, gamma, beta, mean,
-                           inv_std, sums, planes, pixels, channels, cg);
+    const GnFirst g = {images * channels, pixels, channels, cg, make_fastdiv((uint32_t)pixels)};
+    return with_plane<T>(pixels, aligned16(x) && aligned16(dy) && aligned16(dx), [&](auto pack, auto threads) {
+        constexpr int V = decltype(pack)::value, N = decltype(threads)::value;
+        const long blocks = plane_blocks(g.planes, N);
+        if (too_many(blocks)) return PYDTNN_HIP_ERR_UNSUPPORTED;
+        A* ab = sums + 2 * g.planes;
+        hipLaunchKernelGGL((gn_first_bwd_sums<T, V, N, ACT>), dim3((unsigned)blocks), dim3(kT), 0, st, dy, x, gamma, beta, mean,
+                           inv_std, sums, g);
         params(images);
-        if (!dx) return;
-        hipLaunchKernelGGL((gn_bwd_groups<A>), dim3((unsigned)((images * groups + kWaves - 1) / kWaves)), dim3(kT), 0, st, sums,
-                           gamma, ab, images, channels, groups, (double)cg * pixels);
-        hipLaunchKernelGGL((gn_first_bwd_apply<T, N, ACT>), dim3((unsigned)blocks), dim3(kT), 0, st, dy, x, gamma, beta, mean,
-                           inv_std, ab, dx, planes, pixels, channels, cg);
-    };
-    if (small) launch(std::integral_constant<int, kWave>());
-    else launch(std::integral_constant<int, kT>());
-    HIP_RETURN_IF_LAUNCH_FAILED();
-    return PYDTNN_HIP_OK;
+        if (dx) {
+            hipLaunchKernelGGL((gn_bwd_groups<A>), dim3((unsigned)((images * groups + kWaves - 1) / kWaves)), dim3(kT), 0, st,
+                               sums, gamma, ab, images, channels, groups, (double)cg * pixels);
+            hipLaunchKernelGGL((gn_first_bwd_apply<T, V, N, ACT>), dim3((unsigned)blocks), dim3(kT), 0, st, dy, x, gamma, beta,
+                               mean, inv_std, ab, dx, g);
+        }
+        HIP_RETURN_IF_LAUNCH_FAILED();
+        return PYDTNN_HIP_OK;
+    });
 }
 
 }  // namespace
