@@ -184,20 +184,22 @@ __device__ __forceinline__ v8i join(v4i a, v4i b)
     return v8i{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
-// A word of four blocks of 16 rows: a lane's two pieces of each block, and the four scale bytes.  (What it reads of blocks
-// behind the last of a row is not used.)
+// A word of four blocks of 16 rows: a lane's two pieces of each block, and the four scale bytes.  Blocks behind the last are
+// not used: of buffers that one is read again, since an offset beyond a buffer's end would be outside its range check; local
+// memory holds something there.
 struct WordOfBlocks {
     v4i q[4][2];
     int e;
 
-    // `at`: a lane's offset in bytes, of its row and piece; `scale_at`: that of its row's scales
-    __device__ __forceinline__ void load(Rows rows, int at, Rows scales, int scale_at, int word)
+    // `at`: a lane's offset in bytes, of its row and piece; `scale_at`: that of its row's scales; `last`: a row's last block
+    __device__ __forceinline__ void load(Rows rows, int at, Rows scales, int scale_at, int word, int last)
     {
         e = __builtin_amdgcn_raw_buffer_load_b32(scales, scale_at, word * 4, 0);
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-            q[b][0] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rows, at, (word * 4 + b) * kBlock, 0));
-            q[b][1] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rows, at + 64, (word * 4 + b) * kBlock, 0));
+            const int from = min(word * 4 + b, last) * kBlock;
+            q[b][0] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rows, at, from, 0));
+            q[b][1] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rows, at + 64, from, 0));
         }
     }
     __device__ __forceinline__ void load(const uint8_t* row, const uint8_t* scales, int word)
@@ -237,7 +239,7 @@ __global__ void __launch_bounds__(kFewWaves* kWave) matmul_fp8_few_kernel(const 
     WordOfBlocks w[DEPTH], v[LOCAL ? 1 : DEPTH];
 #pragma unroll
     for (int d = 0; d < DEPTH - 1; ++d)
-        if (d < mine) w[d].load(wrows, at, wscales, scale_at, word_of(d));
+        if (d < mine) w[d].load(wrows, at, wscales, scale_at, word_of(d), s.blocks - 1);
     const long stride = kp + 16 + (s.words * 4 + 15) / 16 * 16;
     // rows behind the last are that one again in local memory, zeros otherwise
     const uint8_t* xlocal = local + min((long)row, s.m - 1) * stride;
@@ -255,7 +257,7 @@ __global__ void __launch_bounds__(kFewWaves* kWave) matmul_fp8_few_kernel(const 
     } else {
 #pragma unroll
         for (int d = 0; d < DEPTH - 1; ++d)
-            if (d < mine) v[d].load(xrows, at, xscales, scale_at, word_of(d));
+            if (d < mine) v[d].load(xrows, at, xscales, scale_at, word_of(d), s.blocks - 1);
     }
     for (int done = 0; done < mine; done += DEPTH) {
 #pragma unroll
@@ -263,9 +265,9 @@ __global__ void __launch_bounds__(kFewWaves* kWave) matmul_fp8_few_kernel(const 
             if (done + d >= mine) break;
             const int ahead = word_of(done + d + DEPTH - 1), word = word_of(done + d);
             const bool more = done + d + DEPTH - 1 < mine;
-            if (more) w[(d + DEPTH - 1) % DEPTH].load(wrows, at, wscales, scale_at, ahead);
+            if (more) w[(d + DEPTH - 1) % DEPTH].load(wrows, at, wscales, scale_at, ahead, s.blocks - 1);
             if constexpr (LOCAL) v[0].load(xlocal + piece * 16, xlocal + kp + 16, word);
-            else if (more) v[(d + DEPTH - 1) % DEPTH].load(xrows, at, xscales, scale_at, ahead);
+            else if (more) v[(d + DEPTH - 1) % DEPTH].load(xrows, at, xscales, scale_at, ahead, s.blocks - 1);
             const WordOfBlocks& here = v[LOCAL ? 0 : d];
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
@@ -299,13 +301,13 @@ __global__ void __launch_bounds__(kFewWaves* kWave) matmul_fp8_few_kernel(const 
 // 4096 x 4096: 75 us that way).  There is no output register; what waits for them is wait_loads and the barrier behind it.
 __device__ __forceinline__ void load_quads(uint32_t to, uint32_t at, RowsWords rows, int offset)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(at), "s"(rows), "s"(offset)
-                 : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 ::"s"(to), "v"(at), "s"(rows), "s"(offset) : "memory", "m0");
 }
 __device__ __forceinline__ void load_words(uint32_t to, uint32_t at, RowsWords rows, int offset)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(to), "v"(at), "s"(rows), "s"(offset)
-                 : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
+                 ::"s"(to), "v"(at), "s"(rows), "s"(offset) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 
@@ -314,10 +316,11 @@ __device__ __forceinline__ uint32_t local_address(const void* p)
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
 
+// Waits for all but the last N loads, and for this wave's reads of local memory, whose place the other waves' loads take next.
 template <int N>
 __device__ __forceinline__ void wait_loads()
 {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
 // Writes a tile through local memory, so that whole lines of rows go out: lanes hold four n of 16 different m each (the tile of
@@ -411,15 +414,16 @@ __global__ void __launch_bounds__(WN* WM* kWave, STAGES * (BN + BM) * kBlock > 8
         const int r = (wave + (i < WLOADS ? i : i - WLOADS) * WAVES) * 8 + lane / 8;
         from[i] = (uint32_t)(r * kp) + (uint32_t)(((lane % 8) ^ (lane / 8)) * 16);
     }
-    // the scale words of W's rows, then of x's, 64 rows to a load
+    // the scale words of W's rows, then of x's, 64 rows to a load; where all of those are behind the last, one row is left
+    // to read, since an offset beyond a buffer's end would be outside its range check
     RowsWords scale_from[EACH];
     const uint32_t scale_at = (uint32_t)(lane * s.words * 4);
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
         const int chunk = wave + e * WAVES;
         const bool of_w = chunk < BN / 64;
-        const long r = of_w ? n0 + chunk * 64 : m0 + (chunk - BN / 64) * 64, left = max((of_w ? s.n : s.m) - r, 0l);
-        scale_from[e] = rows_words((of_w ? ws : xs) + (left ? r : 0) * s.words, left * s.words * 4);
+        const long r = of_w ? n0 + chunk * 64 : m0 + (chunk - BN / 64) * 64, left = (of_w ? s.n : s.m) - r;
+        scale_from[e] = rows_words((of_w ? ws : xs) + (left > 0 ? r : 0) * s.words, max(left, 1l) * s.words * 4);
     }
     const uint32_t lds_at = local_address(lds), scales_at = local_address(scale);
     auto load_rows = [&](int step, int stage, int i) {
@@ -504,7 +508,7 @@ __global__ void __launch_bounds__(WN* WM* kWave, STAGES * (BN + BM) * kBlock > 8
 
     if (splits == 1) {
         store_tile<T, BN, BM, TN, TM, WAVES>(lds, acc, wn, wm, y, m0, n0, s, bias, relu);
-    } else if constexpr (BN * BM * 4 <= STAGES * STAGE) {
+    } else if constexpr (BN == 64) {      // (larger tiles are enough by themselves)
         store_tile<float, BN, BM, TN, TM, WAVES>(lds, acc, wn, wm, partial + split * s.m * s.n, m0, n0, s, nullptr, 0);
     }
 }
@@ -550,9 +554,9 @@ Tiling tiling_of(const Fp8Shape& s, bool exact)
     if (!exact && tiles(256) >= 192) t.size = 256;
     else if (tiles(128) >= 192) t.size = 128;
     const long count = tiles(t.size);
-    if (count < 256 && t.size < 256) {
+    if (t.size == 64) {
         long splits = 256 / count;
-                if (splits > s.words / 2) splits = s.words / 2;
+        if (splits > s.words / 2) splits = s.words / 2;
         if (splits > kSplitsMost) splits = kSplitsMost;
         if (splits > 1) t.splits = (int)splits;
     }

@@ -418,6 +418,35 @@ def test_matmul_fp8(ops, shape, dtype):
         assert torch.equal(y, ops.matmul_fp8(misaligned(x), wq, ws, bias=b, relu=relu))
 
 
+@pytest.mark.parametrize("shape", [(1, 17, 33000), (16, 33, 2500), (17, 24577, 640), (40, 24600, 1100)], ids=str)
+@pytest.mark.parametrize("dtype", FP8_DTYPES, ids=str)
+def test_matmul_fp8_at_the_ends_of_its_operands(ops, shape, dtype):
+    """Tiles that hold one row of the weights, or rows of x whose other half is behind the last; words of one to three
+    blocks."""
+    announce("matmul_fp8 ends", shape, dtype)
+    m, n, k = shape
+    x, w = fp8_matrix(m, k, dtype, 1), fp8_matrix(n, k, torch.float32, 2) * 2.0 ** -9
+    wq, ws = ops.quantize_fp8(w)
+    hq, he = oo.quantize_fp8(oo.host64(w))
+    ref, bound = oo.matmul_fp8(oo.host64(x), hq, he, None, False, dtype)
+    within(ops.matmul_fp8(x, wq, ws), ref, bound, "y")
+
+
+@pytest.mark.parametrize("m", [3, 60])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("up", [-120, 126])
+def test_matmul_fp8_with_scales_at_both_ends(ops, m, dtype, up):
+    """Values of one sign and size, whose scales are 2^-127 and 2^118, against weights that bring the product back."""
+    announce("matmul_fp8 scales", m, dtype, up)
+    g = torch.Generator().manual_seed(m)
+    x = ((1 + torch.rand(m, 300, generator=g).double() * 0.9) * 2.0 ** up).to(dtype).cuda()
+    w = ((1 + torch.rand(70, 300, generator=g).double() * 0.9) * 2.0 ** (-up * 5 // 6)).float().cuda()
+    wq, ws = ops.quantize_fp8(w)
+    hq, he = oo.quantize_fp8(oo.host64(w))
+    ref, bound = oo.matmul_fp8(oo.host64(x), hq, he, None, False, dtype)
+    within(ops.matmul_fp8(x, wq, ws), ref, bound, "y")
+
+
 def test_matmul_fp8_keeps_what_is_not_a_number_in_its_row(ops):
     announce("matmul_fp8 NaN")
     for m in (5, 200):
