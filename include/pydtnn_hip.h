@@ -449,7 +449,8 @@ int pydtnn_hip_bn_training_bwd_f64(const double *dy, const double *xn, const dou
  *   backward: from dy, x and the forward's mean and inv_std: dgamma, dbeta (channels) and, unless it is NULL, dx.
  *             Where the activation is PYDTNN_HIP_ACT_RELU, dy counts where z, computed from these inputs, is positive.
  * Sums are taken in a fixed order.  Outputs may not overlap inputs.  channels has to be a multiple of groups; pixels and
- * channels are at most 2^30 (PYDTNN_HIP_ERR_UNSUPPORTED).  Workspace, aligned to 16 bytes: pydtnn_hip_gn_workspace_bytes(...)
+ * channels are at most 2^30, and a launch has fewer than 2^32 threads (PYDTNN_HIP_ERR_UNSUPPORTED: more than 2^26 channels in
+ * the backward pass, for one).  Workspace, aligned to 16 bytes: pydtnn_hip_gn_workspace_bytes(...)
  * with the same extents; backward = 0 or 1; aligned: whether x, y (x, dy and dx) start on multiples of 16 bytes.  Where the
  * forward pass needs none (0) it may be NULL. */
 #define PYDTNN_HIP_ACT_IDENTITY 0
@@ -485,7 +486,8 @@ int pydtnn_hip_dropout(int dtype, const void *x, void *y, long total, double rat
  *       the way and wq (n, kp), wscales as pydtnn_hip_quantize_fp8 makes them of the (n, k) weights, once.  bias (n) is
  *       float32 or NULL; sums are held in float32.
  * x and y are float32, float16 or bfloat16 (`dtype`; PYDTNN_HIP_ERR_INVALID for float64).  q and the workspace are aligned to
- * 16 bytes, scales to 4.  m and n are at most 2^30, k at most 2^23.  Workspace:
+ * 16 bytes, scales to 4.  m and n are at most 2^30, k at most 2^23.  For float32 results the dequantised values go through
+ * bfloat16: those of 2^128 are infinite, and those under 2^-126 may count as 0.  Workspace:
  * pydtnn_hip_matmul_fp8_workspace_bytes(dtype, m, n, k). */
 int pydtnn_hip_quantize_fp8(int dtype, const void *x, long rows, long k, uint8_t *q, uint8_t *scales, void *stream);
 size_t pydtnn_hip_matmul_fp8_workspace_bytes(int dtype, long m, long n, long k);

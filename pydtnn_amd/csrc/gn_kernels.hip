@@ -1329,6 +1329,9 @@ int pydtnn_hip_gn_backward(int dtype, int nhwc, const void* dy, const void* x, c
     const size_t need = pydtnn_hip_gn_workspace_bytes(dtype, nhwc, 1, images, channels, pixels, groups,
                                                       aligned16(x) && aligned16(dy) && aligned16(dx));
     if (!workspace || !aligned16(workspace) || workspace_bytes < need) return PYDTNN_HIP_ERR_WORKSPACE;
+    // (the kernels of channels and of groups; those of x count their own)
+    if (too_many((channels + kParamChannels - 1) / kParamChannels) || (!nhwc && too_many((images * groups + kWaves - 1) / kWaves)))
+        return PYDTNN_HIP_ERR_UNSUPPORTED;
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         using A = wide_t<T>;

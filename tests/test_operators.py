@@ -82,6 +82,19 @@ def test_gn_refuses_extents_it_cannot_run(lib):
     assert lib.pydtnn_hip_gn_backward(0, 1, p, p, p, p, p, p, p, p, p, 2, 8, 4, 2, 0, p, 8, None) == 2
 
 
+@pytest.mark.parametrize("nhwc", [0, 1])
+def test_gn_refuses_launches_of_too_many_threads(lib, nhwc):
+    """Images of one pixel of very many channels, in groups of one: the kernels of the channels and of the groups would have
+    2^32 threads and more.  (The workspace is never touched.)"""
+    p = ctypes.c_void_p(FAKE)
+    for images, channels in ((1, 1 << 26), (1, 1 << 30), (1 << 12, 1 << 14)):
+        need = lib.pydtnn_hip_gn_workspace_bytes(0, nhwc, 1, images, channels, 1, channels, 1)
+        if nhwc and channels == 1 << 14:
+            continue                                      # (runs)
+        assert lib.pydtnn_hip_gn_backward(0, nhwc, p, p, p, p, p, p, p, p, p, images, channels, 1, channels, 0, p, need,
+                                          None) == 4
+
+
 def test_dropout_refuses_rates_and_types_it_does_not_know(lib):
     p = ctypes.c_void_p(FAKE)
     for rate in (-0.1, 1.1, float("nan")):
