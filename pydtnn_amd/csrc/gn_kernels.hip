@@ -12,6 +12,7 @@
 // Every pass is two steps: sums of pieces of each group, then the map with the joined sums.  Sums are held in 32 bits
 // (64 for double), as (mean, sum of squared differences from it) of a piece, and pieces are joined in double through
 // their common mean, so that a mean far from zero costs no digits of the variance.
+#include <algorithm>
 #include <cmath>
 #include "../../include/pydtnn_hip.h"
 #include "conv_internal.h"
@@ -827,7 +828,8 @@ template <typename T, int V, int ACT, int THREADS, int PACKS>
 __global__ void __launch_bounds__(THREADS) gn_first_whole(const T* __restrict__ x, const wide_t<T>* __restrict__ gamma,
                                                           const wide_t<T>* __restrict__ beta, T* __restrict__ y,
                                                           wide_t<T>* __restrict__ mean_out,
-                                                          wide_t<T>* __restrict__ inv_std_out, double eps, GnFirst g, GnLast join)
+                                                          wide_t<T>* __restrict__ inv_std_out, double eps, GnFirst g,
+                                                          GnLast join)
 {
     using A = wide_t<T>;
     __shared__ A mean, inv_std;
@@ -998,9 +1000,9 @@ GnLast last_shape(long images, int channels, int pixels, int groups, int v)
     g.slabs = groups / g.slab_groups;
     const int packs = g.width / v;
     g.tx = packs < kT ? packs : kT;
-    g.rows = kT / g.tx;
-    // three workgroups to each of 256 compute units, which hold them all at once (backward 64 x 56 x 56 x 256 in float32: 182 us
-    // against 188 with four and 199 with eight), and at least eight pixels to a thread
+    g.rows = std::min(kT / g.tx, pixels);
+    // three workgroups to each of 256 compute units, which hold them all at once (backward 64 x 56 x 56 x 256 in float32: 178
+    // us against 188 with four and 199 with eight), and at least eight pixels to a thread
     long want = (768 + images * g.slabs - 1) / (images * g.slabs);
     const long most = (pixels + 8l * g.rows - 1) / (8l * g.rows);
     if (want > most) want = most;
@@ -1026,7 +1028,7 @@ bool whole_shape(GnLast* g, long images, int channels, int pixels, int groups, i
         // a slab of few packs leaves threads idle: it grows while there are workgroups enough
         if (2l * pixels * tx < threads * packs && sg != groups && images * (groups / sg) > 1024) continue;
         if (tx > threads || (pixels + threads / tx - 1) / (threads / tx) > packs) break;
-        *g = GnLast{images, pixels, channels, groups, cg, sg, width, groups / sg, tx, threads / tx, 1, pixels,
+        *g = GnLast{images, pixels, channels, groups, cg, sg, width, groups / sg, tx, std::min(threads / tx, pixels), 1, pixels,
                     images * (groups / sg), 1, 1, {}};
         set_joins(g, threads, v);
         return g->pieces <= most && (g->pieces + 8) * threads < (1l << 32);      // (a launch counts its threads in 32 bits)
@@ -1049,12 +1051,16 @@ int size_of(int dtype) { return dtype == kDtypeF64 ? 8 : dtype == kDtypeF32 ? 4 
 // (forward 16 x 28 x 28 x 512 in bfloat16: 12 us and 15) and whole lines of 128 bytes before half lines
 // (forward 64 x 14 x 14 x 1024 in float32: 19 us with lines, 22 with half lines).  The largest workgroup has a compute unit
 // to itself and is taken where one round of them does it all: forward 56 x 56 x 256 in float32 takes 22 us against 30 in two
-// passes for 16 images (256 slabs), 103 against 102 for 64.
+// passes for 16 images (256 slabs), 103 against 102 for 64.  Where the images' rows of `rows_bytes` in all make fewer than 256
+// whole lines, slabs are narrower, so that more compute units have one: caches hold tensors this small (4 x 28 x 28 x 128 in
+// bfloat16: forward 10 -> 9 us, backward 16 -> 12).
 template <int FEW, int SOME_THREADS, int SOME, int MANY_THREADS, int MANY, typename F>
-bool hold_slabs(F launch)
+bool hold_slabs(long rows_bytes, F launch)
 {
     using std::integral_constant;
-    for (int line = 128; line >= 64; line /= 2)
+    int first = 128;
+    while (first > 16 && rows_bytes / first < 256) first /= 2;
+    for (int line = first; line >= std::min(first, 64); line /= 2)
         if (launch(line, 1l << 40, integral_constant<int, 256>(), integral_constant<int, FEW>()) ||
             launch(line, 1l << 40, integral_constant<int, SOME_THREADS>(), integral_constant<int, SOME>()))
             return true;
@@ -1065,15 +1071,15 @@ bool hold_slabs(F launch)
 
 // SHORT: packs of eight 16-bit values, which leave room for fewer threads.
 template <bool SHORT, typename F>
-bool hold_forward(F launch)
+bool hold_forward(long rows_bytes, F launch)
 {
-    return hold_slabs<4, 512, 8, SHORT ? 512 : 1024, SHORT ? 24 : 16>(launch);
+    return hold_slabs<4, 512, 8, SHORT ? 512 : 1024, SHORT ? 24 : 16>(rows_bytes, launch);
 }
 
 template <bool SHORT, typename F>
-bool hold_backward(F launch)
+bool hold_backward(long rows_bytes, F launch)
 {
-    return hold_slabs<4, SHORT ? 256 : 512, 8, SHORT ? 512 : 1024, SHORT ? 12 : 8>(launch);
+    return hold_slabs<4, SHORT ? 256 : 512, 8, SHORT ? 512 : 1024, SHORT ? 12 : 8>(rows_bytes, launch);
 }
 
 // Calls launch(threads, packs) for the smallest workgroup whose registers hold `packs` packs of a group that is one run of
@@ -1110,7 +1116,8 @@ size_t workspace_bytes_of(int dtype, bool nhwc, bool backward, long images, int 
             GnLast g;
             return whole_shape(&g, images, channels, pixels, groups, v, size, line, most, threads, packs);
         };
-        if (!backward && (size == 2 ? hold_forward<true>(fits) : hold_forward<false>(fits))) return 0;
+        const long rows_bytes = images * channels * size;
+        if (!backward && (size == 2 ? hold_forward<true>(rows_bytes, fits) : hold_forward<false>(rows_bytes, fits))) return 0;
         const GnLast g = last_shape(images, channels, pixels, groups, v);
         moments = images * groups * g.splits;
         sums = images * channels * g.splits;
@@ -1181,7 +1188,7 @@ int forward(int nhwc, const T* x, const wide_t<T>* gamma, const wide_t<T>* beta,
                                gamma, beta, y, mean, inv_std, eps, g);
             return true;
         };
-        if (hold_forward<sizeof(T) == 2>(whole)) {
+        if (hold_forward<sizeof(T) == 2>(images * channels * (long)sizeof(T), whole)) {
             HIP_RETURN_IF_LAUNCH_FAILED();
             return PYDTNN_HIP_OK;
         }
@@ -1247,7 +1254,7 @@ int backward(int nhwc, const T* dy, const T* x, const wide_t<T>* gamma, const wi
             params(images);
             return true;
         };
-        if (hold_backward<sizeof(T) == 2>(whole)) {
+        if (hold_backward<sizeof(T) == 2>(images * channels * (long)sizeof(T), whole)) {
             HIP_RETURN_IF_LAUNCH_FAILED();
             return PYDTNN_HIP_OK;
         }
@@ -1330,7 +1337,8 @@ int pydtnn_hip_gn_backward(int dtype, int nhwc, const void* dy, const void* x, c
                                                       aligned16(x) && aligned16(dy) && aligned16(dx));
     if (!workspace || !aligned16(workspace) || workspace_bytes < need) return PYDTNN_HIP_ERR_WORKSPACE;
     // (the kernels of channels and of groups; those of x count their own)
-    if (too_many((channels + kParamChannels - 1) / kParamChannels) || (!nhwc && too_many((images * groups + kWaves - 1) / kWaves)))
+    if (too_many((channels + kParamChannels - 1) / kParamChannels) ||
+        (!nhwc && too_many((images * groups + kWaves - 1) / kWaves)))
         return PYDTNN_HIP_ERR_UNSUPPORTED;
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
