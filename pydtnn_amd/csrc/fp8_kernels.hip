@@ -272,8 +272,8 @@ __global__ void __launch_bounds__(kFewWaves* kWave) matmul_fp8_few_kernel(const 
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 if (word * 4 + b >= s.blocks) break;
-                acc = block_product<EXACT>(join(w[d].q[b][0], w[d].q[b][1]), w[d].e >> (8 * b), join(here.q[b][0], here.q[b][1]),
-                                           here.e >> (8 * b), acc);
+                acc = block_product<EXACT>(join(w[d].q[b][0], w[d].q[b][1]), w[d].e >> (8 * b),
+                                           join(here.q[b][0], here.q[b][1]), here.e >> (8 * b), acc);
             }
         }
     }
@@ -333,6 +333,7 @@ __device__ __forceinline__ void store_tile(uint8_t* lds, const v4f (&acc)[TN][TM
     constexpr int PER = 16 / (int)sizeof(T), PIECES = BN / PER;      // elements of a piece, pieces of a row
     constexpr int TURNS = PIECES < 16 ? PIECES : 16;
     const int lane = threadIdx.x % kWave, row = lane % 16, piece = lane / 16;
+    auto place = [&](int m, int n) { return lds + m * BN * sizeof(T) + ((n / PER) ^ (m % TURNS)) * 16; };
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < TN; ++i) {
@@ -353,7 +354,7 @@ __device__ __forceinline__ void store_tile(uint8_t* lds, const v4f (&acc)[TN][TM
                 if (relu) v = v > 0.0f ? v : 0.0f;
                 out.v[k] = (T)v;
             }
-            *reinterpret_cast<Pack<T, 4>*>(lds + m * BN * sizeof(T) + ((n / PER) ^ (m % TURNS)) * 16 + n % PER * sizeof(T)) = out;
+            *reinterpret_cast<Pack<T, 4>*>(place(m, n) + n % PER * sizeof(T)) = out;
         }
     }
     __syncthreads();
@@ -362,7 +363,7 @@ __device__ __forceinline__ void store_tile(uint8_t* lds, const v4f (&acc)[TN][TM
     for (int at = threadIdx.x; at < BM * PIECES; at += WAVES * kWave) {
         const int m = at / PIECES, n = at % PIECES * PER;
         if (m0 + m >= s.m || n0 + n >= s.n) continue;
-        const Pack<T, PER> v = *reinterpret_cast<const Pack<T, PER>*>(lds + m * BN * sizeof(T) + ((n / PER) ^ (m % TURNS)) * 16);
+        const Pack<T, PER> v = *reinterpret_cast<const Pack<T, PER>*>(place(m, n));
         T* to = y + (m0 + m) * s.n + n0 + n;
         if (whole) {
             // past the caches: the workgroups of a launch store all at once (4096 x 4096 in bfloat16: 13 us, plain stores 19)
@@ -497,7 +498,8 @@ __global__ void __launch_bounds__(WN* WM* kWave, STAGES * (BN + BM) * kBlock > 8
             // a coming step's loads, a few at a time over the first half of the products
             if (coming < last) {
 #pragma unroll
-                for (int l = i * 2 * LOADS / TN; l < (i + 1) * 2 * LOADS / TN && l < LOADS; ++l) load_rows(coming, coming_stage, l);
+                for (int l = i * 2 * LOADS / TN; l < (i + 1) * 2 * LOADS / TN && l < LOADS; ++l)
+                    load_rows(coming, coming_stage, l);
             }
 #pragma unroll
             for (int j = 0; j < TM; ++j) acc[i][j] = block_product<EXACT>(w, we[i], x[j], xe[j], acc[i][j]);
@@ -611,14 +613,15 @@ int launch_tiles(const uint8_t* xq, const uint8_t* xs, const uint8_t* wq, const 
     const long tiles_n = (s.n + BN - 1) / BN, tiles_m = (s.m + BM - 1) / BM;
     const long blocks = (tiles_n * tiles_m * splits + 7) / 8 * 8;
     if (blocks * WN * WM * kWave >= (1l << 32)) return PYDTNN_HIP_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((matmul_fp8_tile_kernel<T, EXACT, BN, BM, WN, WM, STAGES>), dim3((unsigned)blocks), dim3(WN * WM * kWave),
-                       0, st, xq, (const uint32_t*)xs, wq, (const uint32_t*)ws, bias, y, partial, s, relu, (int)tiles_n,
-                       (int)tiles_m, splits);
+    hipLaunchKernelGGL((matmul_fp8_tile_kernel<T, EXACT, BN, BM, WN, WM, STAGES>), dim3((unsigned)blocks),
+                       dim3(WN * WM * kWave), 0, st, xq, (const uint32_t*)xs, wq, (const uint32_t*)ws, bias, y, partial, s, relu,
+                       (int)tiles_n, (int)tiles_m, splits);
     HIP_RETURN_IF_LAUNCH_FAILED();
     if (splits == 1) return PYDTNN_HIP_OK;
     const long join = (s.m * s.n + kT - 1) / kT;
     if (join * kT >= (1l << 32)) return PYDTNN_HIP_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((join_splits_kernel<T>), dim3((unsigned)join), dim3(kT), 0, st, partial, bias, y, s.m, s.n, splits, relu);
+    hipLaunchKernelGGL((join_splits_kernel<T>), dim3((unsigned)join), dim3(kT), 0, st, partial, bias, y, s.m, s.n, splits,
+                       relu);
     HIP_RETURN_IF_LAUNCH_FAILED();
     return PYDTNN_HIP_OK;
 }
@@ -631,14 +634,14 @@ int product(const T* x, const uint8_t* xq, const uint8_t* xs, const uint8_t* wq,
     if (s.m <= kFewRows) {
         const long blocks = (s.n + 15) / 16;
         if (blocks * kFewWaves * kWave >= (1l << 32)) return PYDTNN_HIP_ERR_UNSUPPORTED;
-        auto few = [&](auto depth, auto local, auto packed) {
-            hipLaunchKernelGGL((matmul_fp8_few_kernel<T, decltype(depth)::value, decltype(local)::value, decltype(packed)::value>),
+        auto few = [&](auto local, auto packed) {
+            hipLaunchKernelGGL((matmul_fp8_few_kernel<T, 2, decltype(local)::value, decltype(packed)::value>),
                                dim3((unsigned)blocks), dim3(kFewWaves * kWave), 0, st, x, xq, (const uint32_t*)xs, wq,
                                (const uint32_t*)ws, bias, y, s, relu);
         };
-        if (!few_local(s)) few(std::integral_constant<int, 2>(), std::false_type(), std::false_type());
-        else if (aligned16(x) && s.k % 8 == 0) few(std::integral_constant<int, 2>(), std::true_type(), std::true_type());
-        else few(std::integral_constant<int, 2>(), std::true_type(), std::false_type());
+        if (!few_local(s)) few(std::false_type(), std::false_type());
+        else if (aligned16(x) && s.k % 8 == 0) few(std::true_type(), std::true_type());
+        else few(std::true_type(), std::false_type());
         HIP_RETURN_IF_LAUNCH_FAILED();
         return PYDTNN_HIP_OK;
     }
@@ -646,7 +649,8 @@ int product(const T* x, const uint8_t* xq, const uint8_t* xs, const uint8_t* wq,
     if constexpr (!EXACT)
         if (t.size == 256)
             return launch_tiles<T, EXACT, 256, 256, 2, 4, 2>(xq, xs, wq, ws, bias, y, partial, s, relu, t.splits, st);
-    if (t.size == 128) return launch_tiles<T, EXACT, 128, 128, 2, 2, 2>(xq, xs, wq, ws, bias, y, partial, s, relu, t.splits, st);
+    if (t.size == 128)
+        return launch_tiles<T, EXACT, 128, 128, 2, 2, 2>(xq, xs, wq, ws, bias, y, partial, s, relu, t.splits, st);
     return launch_tiles<T, EXACT, 64, 64, 2, 2, 4>(xq, xs, wq, ws, bias, y, partial, s, relu, t.splits, st);
 }
 

@@ -540,21 +540,22 @@ def _wide(dtype):
     return torch.float64 if dtype == torch.float64 else torch.float32
 
 
-def _need_like(x, dtype, **tensors):
-    """Each (tensor, shape) is of type ``dtype``, of that shape and on the device of ``x``."""
-    for name, (t, shape) in tensors.items():
+def _need_like(x, dtype, shape, **tensors):
+    """Each tensor is of type ``dtype``, of shape ``shape`` (a tuple) and on the device of ``x``."""
+    device = x.device
+    for name, t in tensors.items():
         if t.dtype != dtype:
             raise TypeError(f"{name} is {t.dtype}, {dtype} expected")
-        if tuple(t.shape) != tuple(shape):
+        if t.shape != shape:
             raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-        if t.device != x.device:
-            raise ValueError(f"{name} is on {t.device}, the other tensors on {x.device}")
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
 
 
 def _scratch(nbytes, x):
     """Scratch memory of one call, None for no bytes.  It is the call's alone: under capture it belongs to the graph that
     is captured, and no other graph or later call is handed the same memory while this one can still run."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    return x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 _GN_ACTIVATIONS = {"": 0, None: 0, "relu": 1, "silu": 2}
@@ -569,15 +570,16 @@ def _gn_extents(x, gamma, beta, groups, activation, nhwc):
     channels = x.shape[-1] if nhwc else x.shape[1]
     if groups < 1 or channels < 1 or channels % groups:
         raise ValueError(f"{channels} channels do not make {groups} groups")
-    _need_like(x, _wide(x.dtype), gamma=(gamma, (channels,)), beta=(beta, (channels,)))
-    pixels = math.prod(x.shape[1:]) // channels
+    _need_like(x, _wide(x.dtype), (channels,), gamma=gamma, beta=beta)
+    images = x.shape[0]
+    pixels = (x.numel() // images if images else math.prod(x.shape[1:])) // channels
     if pixels < 1:
         raise ValueError(f"group normalisation of no pixels: x has shape {tuple(x.shape)}")
-    return x.shape[0], channels, pixels, groups, _GN_ACTIVATIONS[activation]
+    return images, channels, pixels, groups, _GN_ACTIVATIONS[activation]
 
 
-def _is_aligned(*tensors):
-    return all(t.data_ptr() % 16 == 0 for t in tensors)
+def _is_aligned(a, b):
+    return not (a.data_ptr() | b.data_ptr()) & 15
 
 
 @_on_its_device
@@ -592,14 +594,14 @@ def gn_forward(x, gamma, beta, groups, eps=1e-5, activation="", nhwc=True):
         raise ValueError(f"epsilon is {eps}, it has to be at least 0")
     x = x.contiguous()
     y = torch.empty_like(x)
-    mean = torch.empty((images, groups), dtype=gamma.dtype, device=x.device)
+    mean = gamma.new_empty((images, groups))
     inv_std = torch.empty_like(mean)
     if images:
         nbytes = lib().pydtnn_hip_gn_workspace_bytes(dtype, int(nhwc), 0, images, channels, pixels, groups,
                                                      _is_aligned(x, y))
         ws = _scratch(nbytes, x)
-        check(lib().pydtnn_hip_gn_forward(dtype, int(nhwc), address(x), address(gamma), address(beta), address(y),
-                                          address(mean), address(inv_std), images, channels, pixels, groups, float(eps),
+        check(lib().pydtnn_hip_gn_forward(dtype, int(nhwc), address(x), address(gamma), address(beta), y.data_ptr(),
+                                          mean.data_ptr(), inv_std.data_ptr(), images, channels, pixels, groups, float(eps),
                                           act, address(ws), nbytes, raw_stream(x)), "gn_forward")
     return y, mean, inv_std
 
@@ -609,8 +611,8 @@ def gn_backward(dy, x, gamma, beta, mean, inv_std, groups, activation="", nhwc=T
     """The gradients of ``gn_forward`` from its input and its two statistics -> (dgamma, dbeta, dx or None)."""
     dtype = _dtype_of(x)
     images, channels, pixels, groups, act = _gn_extents(x, gamma, beta, groups, activation, nhwc)
-    _need_like(x, x.dtype, dy=(dy, x.shape))
-    _need_like(x, gamma.dtype, mean=(mean, (images, groups)), inv_std=(inv_std, (images, groups)))
+    _need_like(x, x.dtype, x.shape, dy=dy)
+    _need_like(x, gamma.dtype, (images, groups), mean=mean, inv_std=inv_std)
     dy, x = dy.contiguous(), x.contiguous()
     dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(gamma)
     dx = torch.empty_like(x) if need_dx else None
@@ -647,7 +649,7 @@ def dropout(x, rate, seed, offset=0):
     y = torch.empty_like(x)
     if x.numel():
         mask = (1 << 64) - 1
-        check(lib().pydtnn_hip_dropout(dtype, address(x), address(y), x.numel(), float(rate), int(seed) & mask,
+        check(lib().pydtnn_hip_dropout(dtype, address(x), y.data_ptr(), x.numel(), float(rate), int(seed) & mask,
                                        int(offset) & mask, offset_dev, raw_stream(x)), "dropout")
     return y
 
@@ -700,15 +702,15 @@ def matmul_fp8(x, wq, wscales, bias=None, relu=False):
         raise ValueError(f"quantised weights are an (n, k) matrix, not a tensor of shape {tuple(wq.shape)}")
     n = wq.shape[0]
     q_shape, scales_shape = _fp8_shapes(n, k)
-    _need_like(x, torch.float8_e4m3fn, weights=(wq, q_shape))
-    _need_like(x, torch.uint8, scales=(wscales, scales_shape))
+    _need_like(x, torch.float8_e4m3fn, q_shape, weights=wq)
+    _need_like(x, torch.uint8, scales_shape, scales=wscales)
     if bias is not None:
-        _need_like(x, torch.float32, bias=(bias, (n,)))
+        _need_like(x, torch.float32, (n,), bias=bias)
     x = x.contiguous()
-    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    y = x.new_empty((m, n))
     if m:
         nbytes = lib().pydtnn_hip_matmul_fp8_workspace_bytes(dtype, m, n, k)
         ws = _scratch(nbytes, x)
         check(lib().pydtnn_hip_matmul_fp8(dtype, address(x), m, k, address(wq), address(wscales), n, address(bias),
-                                          int(relu), address(y), address(ws), nbytes, raw_stream(x)), "matmul_fp8")
+                                          int(relu), y.data_ptr(), address(ws), nbytes, raw_stream(x)), "matmul_fp8")
     return y
