@@ -176,7 +176,9 @@ __device__ __forceinline__ RowsWords rows_words(const void* base, long bytes)
 // first operand, so that a lane ends with four consecutive n of one m.
 //
 // Where local memory holds all of x (kFewLocal bytes), every workgroup quantises it for itself, while its first weights
-// are on their way: one launch instead of two.  Otherwise x comes quantised.
+// are on their way: one launch instead of two (1 x 4096 x 1000 in float32: 5.8 us, 7.4 with two).  Otherwise x comes quantised.
+// 16 x 4096 x 1000 in float32 takes 9 us, 12 in tiles; 8 x 4096 x 4096 9.5 and 13; 16 x 25088 x 4096 34 and 38, where the
+// weights arrive at 3.6 TB/s beside as many bytes of x from the second-level cache.
 constexpr int kFewWaves = 8, kFewLocal = 32 * 1024;
 
 __device__ __forceinline__ v8i join(v4i a, v4i b)
@@ -540,11 +542,11 @@ size_t scale_bytes(const Fp8Shape& s) { return ((size_t)s.m * s.words * 4 + 15) 
 constexpr long kFewRows = 16;
 constexpr int kSplitsMost = 16;
 
-// Tiles of `size` by `size`: the largest that are about enough for 256 compute units (512 x 4096 x 4096 in bfloat16: 23 us with
-// 256 tiles of 128 by 128 ... 4096 x 4096 x 4096: 73 us with 256 by 256, 86 with 128 by 128).  Where there are fewer, k is cut
-// into `splits` pieces of at least two words of four blocks, a workgroup each, as far as there are units for them (777 x 2049 x
-// 1003 in float16: 15 us with 208 workgroups, 20 with twice as many, whose results have to be joined; 64 x 25088 x 4096: 37
-// and 41).
+// Tiles of `size` by `size`: the largest that are about enough for 256 compute units.  In bfloat16, quantising x included:
+// 4096 x 4096 x 4096 72 us with 256 by 256, 79 with 128 by 128, 123 with 64 by 64; 1024 x 4096 x 4096 35 with 128, 57 with
+// 256, 37 with 64; 512 x 4096 x 4096 23 with 64, 33 with 128.  Where tiles of 64 are too few, k is cut into `splits` pieces of
+// at least two words of four blocks, a workgroup each, as far as there are units for them (777 x 2049 x 1003 in float16: 15 us
+// with 208 workgroups, 20 with twice as many, whose results have to be joined; 64 x 25088 x 4096: 37 and 41).
 struct Tiling {
     int size, splits;
 };
@@ -614,8 +616,8 @@ int launch_tiles(const uint8_t* xq, const uint8_t* xs, const uint8_t* wq, const 
     const long blocks = (tiles_n * tiles_m * splits + 7) / 8 * 8;
     if (blocks * WN * WM * kWave >= (1l << 32)) return PYDTNN_HIP_ERR_UNSUPPORTED;
     hipLaunchKernelGGL((matmul_fp8_tile_kernel<T, EXACT, BN, BM, WN, WM, STAGES>), dim3((unsigned)blocks),
-                       dim3(WN * WM * kWave), 0, st, xq, (const uint32_t*)xs, wq, (const uint32_t*)ws, bias, y, partial, s, relu,
-                       (int)tiles_n, (int)tiles_m, splits);
+                       dim3(WN * WM * kWave), 0, st, xq, (const uint32_t*)xs, wq, (const uint32_t*)ws, bias, y, partial,
+                       s, relu, (int)tiles_n, (int)tiles_m, splits);
     HIP_RETURN_IF_LAUNCH_FAILED();
     if (splits == 1) return PYDTNN_HIP_OK;
     const long join = (s.m * s.n + kT - 1) / kT;

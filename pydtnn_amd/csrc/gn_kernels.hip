@@ -9,9 +9,14 @@
 // The backward pass keeps nothing of the forward pass but x and the two statistics of each group: xn and z are
 // computed again.  Both passes are bound by memory: forward reads x and writes y, backward reads x and dy and writes dx.
 //
-// Every pass is two steps: sums of pieces of each group, then the map with the joined sums.  Sums are held in 32 bits
-// (64 for double), as (mean, sum of squared differences from it) of a piece, and pieces are joined in double through
-// their common mean, so that a mean far from zero costs no digits of the variance.
+// Each is sums of a group, then the map.  Where the registers of a workgroup hold whole groups, one kernel does both and
+// x is read once (..._whole): 16 x 56 x 56 x 256 forward in float32 takes 22 us, 4.8 TB/s.  Elsewhere there are two passes:
+// sums of pieces of each group (moments, bwd_sums), then the map with the joined sums (apply): 64 x 56 x 56 x 256 in float32
+// takes 100 us forward, where a copy takes 76, and 178 backward (114), with 6.1 and 5.8 TB/s moved.  The smallest calls take
+// 5 us, a launch.
+//
+// Sums are held in 32 bits (64 for double), as (mean, sum of squared differences from it) of a piece, and pieces are joined
+// in double through their common mean, so that a mean far from zero costs no digits of the variance.
 #include <algorithm>
 #include <cmath>
 #include "../../include/pydtnn_hip.h"
@@ -710,6 +715,7 @@ __global__ void __launch_bounds__(THREADS) gn_last_bwd_whole(const T* __restrict
 // ---------------------------------------------------------------------------------------------- channels first
 // A group is one run of memory here.  Where a workgroup's registers hold it, one kernel does the forward pass; otherwise, and
 // in the backward pass, whose sums are of channels, THREADS threads take a plane: one channel of one image.
+// 64 x 256 x 56 x 56: forward 88 us in float32 and 55 in bfloat16 (196 and 148 in planes), backward 183 and 92.
 struct GnFirst {
     long planes;                     // images * channels
     int pixels, channels, cg;

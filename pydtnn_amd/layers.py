@@ -664,7 +664,8 @@ class Dropout(Layer):
 
     With a ``seed`` (0 <= seed < 2^32) the mask is a function of the seed, the layer's id and the number of its training
     steps so far, and is stored nowhere: the backward pass draws it again.  ``step`` holds that number on the GPU, counted up
-    by each forward pass in TRAIN_MODE (also by each replay of a captured one); setting it resumes a run where it was."""
+    by each forward pass in TRAIN_MODE (also by each replay of a captured one); filling it in place resumes a run where it
+    was.  The backward pass belongs to the last forward pass; processes that train together each take a seed of their own."""
 
     def __init__(self, rate=0.5, seed=None):
         super().__init__()
