@@ -1052,40 +1052,60 @@ int check(long images, long channels, long pixels, long groups)
 
 int size_of(int dtype) { return dtype == kDtypeF64 ? 8 : dtype == kDtypeF32 ? 4 : 2; }
 
-// Calls launch(line, most, threads, packs) for the ways to hold a slab, the better first, until one fits: few threads before
-// many (several workgroups to a compute unit, whose loads and stores overlap), eight packs to a thread rather than sixteen
-// (forward 16 x 28 x 28 x 512 in bfloat16: 12 us and 15) and whole lines of 128 bytes before half lines
-// (forward 64 x 14 x 14 x 1024 in float32: 19 us with lines, 22 with half lines).  The largest workgroup has a compute unit
-// to itself and is taken where one round of them does it all: forward 56 x 56 x 256 in float32 takes 22 us against 30 in two
-// passes for 16 images (256 slabs), 103 against 102 for 64.  Where the images' rows of `rows_bytes` in all make fewer than 256
-// whole lines, slabs are narrower, so that more compute units have one: caches hold tensors this small (4 x 28 x 28 x 128 in
-// bfloat16: forward 10 -> 9 us, backward 16 -> 12).
-template <int FEW, int SOME_THREADS, int SOME, int MANY_THREADS, int MANY, typename F>
-bool hold_slabs(long rows_bytes, F launch)
+// A way to hold a slab: a workgroup's threads, and the packs that each holds.
+template <int THREADS, int PACKS>
+struct Hold {};
+
+// Calls launch(line, most, threads, packs) for these ways in turn, with whole lines of `first` bytes, then with half lines of
+// 64 (forward 64 x 14 x 14 x 1024 in float32: 19 us with lines of 128, 22 with half lines), until one fits.
+template <typename F, int... THREADS, int... PACKS>
+bool hold_lines(int first, long most, F launch, Hold<THREADS, PACKS>...)
 {
-    using std::integral_constant;
-    int first = 128;
-    while (first > 16 && rows_bytes / first < 256) first /= 2;
     for (int line = first; line >= std::min(first, 64); line /= 2)
-        if (launch(line, 1l << 40, integral_constant<int, 256>(), integral_constant<int, FEW>()) ||
-            launch(line, 1l << 40, integral_constant<int, SOME_THREADS>(), integral_constant<int, SOME>()))
+        if ((launch(line, most, std::integral_constant<int, THREADS>(), std::integral_constant<int, PACKS>()) || ...))
             return true;
-    for (int line = 128; line >= 64; line /= 2)
-        if (launch(line, 256l, integral_constant<int, MANY_THREADS>(), integral_constant<int, MANY>())) return true;
     return false;
 }
 
-// SHORT: packs of eight 16-bit values, which leave room for fewer threads.
+// The lines that slabs are made of.  Where the images' rows, of `rows_bytes` in all, make fewer than 256 whole lines, slabs are
+// narrower, so that more compute units have one: caches hold tensors this small (4 x 28 x 28 x 128 in bfloat16: forward 10 -> 9
+// us, backward 16 -> 12).
+int first_line(long rows_bytes)
+{
+    int first = 128;
+    while (first > 16 && rows_bytes / first < 256) first /= 2;
+    return first;
+}
+
+// The ways to hold slabs, the better first: few threads before many (several workgroups to a compute unit, whose loads and
+// stores overlap) and few packs to a thread before many (forward 16 x 28 x 28 x 512 in bfloat16: 12 us with eight packs to 512
+// threads, 15 with sixteen to 256).  Sixteen packs to 512 threads still beat two passes (forward 64 x 28 x 28 x 512 in float64:
+// 86 us against 104; 64 x 40 x 40 x 256 in float32: 48 against 52), and so do two tensors of eight packs to 1024 (backward:
+// 156 against 187; 92 against 95).  A workgroup that has a compute unit to itself is taken where one round of them does it all:
+// forward 56 x 56 x 256 in float32 takes 22 us against 30 in two passes for 16 images (256 slabs), 103 against 102 for 64.
+// SHORT: packs of eight 16-bit values, whose sums leave registers for fewer of them (backward 64 x 28 x 28 x 512 in bfloat16:
+// 61 us in two passes, 81 with twelve packs to 512 threads).
+constexpr long kAny = 1l << 40, kOneRound = 256;
+
 template <bool SHORT, typename F>
 bool hold_forward(long rows_bytes, F launch)
 {
-    return hold_slabs<4, 512, 8, SHORT ? 512 : 1024, SHORT ? 24 : 16>(rows_bytes, launch);
+    const int line = first_line(rows_bytes);
+    if (hold_lines(line, kAny, launch, Hold<256, 4>(), Hold<512, 8>())) return true;
+    if constexpr (SHORT) return hold_lines(128, kOneRound, launch, Hold<512, 24>());
+    else return hold_lines(line, kAny, launch, Hold<512, 16>()) || hold_lines(128, kOneRound, launch, Hold<1024, 16>());
 }
 
 template <bool SHORT, typename F>
 bool hold_backward(long rows_bytes, F launch)
 {
-    return hold_slabs<4, SHORT ? 256 : 512, 8, SHORT ? 512 : 1024, SHORT ? 12 : 8>(rows_bytes, launch);
+    const int line = first_line(rows_bytes);
+    if constexpr (SHORT)
+        return hold_lines(line, kAny, launch, Hold<256, 4>(), Hold<256, 8>()) ||
+               hold_lines(128, kOneRound, launch, Hold<512, 12>());
+    else
+        return hold_lines(line, kAny, launch, Hold<256, 4>(), Hold<512, 8>()) ||
+               hold_lines(line, kAny, launch, Hold<1024, 8>());
 }
 
 // Calls launch(threads, packs) for the smallest workgroup whose registers hold `packs` packs of a group that is one run of

@@ -110,6 +110,15 @@ def test_group_norm(ops, shape, dtype, nhwc):
         check_gn(ops, *gn_inputs(shape, dtype, nhwc, 5), activation, nhwc)
 
 
+@pytest.mark.parametrize("nhwc", [True, False], ids=["last", "first"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [(64, (13, 17), 128, 8), (64, (23, 23), 128, 4), (30, (18, 17), 544, 17)], ids=str)
+def test_group_norm_of_many_slabs_of_whole_lines(ops, shape, dtype, nhwc):
+    """Images enough for a slab of whole lines to each compute unit, of sizes that take the larger workgroups."""
+    announce("group norm, many slabs", shape, dtype, nhwc)
+    check_gn(ops, *gn_inputs(shape, dtype, nhwc, 6), "silu" if shape[0] == 30 else "relu", nhwc)
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("offset", [100.0, -3000.0])
 def test_group_norm_of_values_far_from_zero(ops, dtype, offset):
