@@ -722,36 +722,73 @@ struct GnFirst {
     FastDiv by_pixels;               // exact for the elements of a group that one kernel holds, at most 2^16
 };
 
-// Calls f(pack of x, its number) for the packs of a plane, kAhead loads under way at once.
-template <int THREADS, typename P, typename F>
-__device__ __forceinline__ void each_pack(const P* x, int packs, F f)
+// V elements that start anywhere: planes of odd extents start off the boundaries of 16 bytes, where loads and stores of 16
+// bytes still beat those of an element.
+template <typename T, int V>
+struct Loose {
+    T v[V];
+};
+
+// Calls f(V elements of x, their first's number) for a plane, kAhead loads under way at once, and then f(one element, its
+// number) for what is left.
+template <int THREADS, int V, typename T, typename F>
+__device__ __forceinline__ void each_pack(const T* x, int pixels, F f)
 {
-    int p = threadIdx.x % THREADS;
-    for (; p + (kAhead - 1) * THREADS < packs; p += kAhead * THREADS) {
+    using P = Loose<T, V>;
+    int p = threadIdx.x % THREADS * V;
+    for (; p + (kAhead - 1) * THREADS * V + V <= pixels; p += kAhead * THREADS * V) {
         P v[kAhead];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) v[u] = x[p + u * THREADS];
+        for (int u = 0; u < kAhead; ++u) __builtin_memcpy(&v[u], x + p + u * THREADS * V, sizeof(P));
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) f(v[u], p + u * THREADS);
+        for (int u = 0; u < kAhead; ++u) f(v[u], p + u * THREADS * V);
     }
-    for (; p < packs; p += THREADS) f(x[p], p);
+    for (; p + V <= pixels; p += THREADS * V) {
+        P v;
+        __builtin_memcpy(&v, x + p, sizeof(P));
+        f(v, p);
+    }
+    p = pixels / V * V + threadIdx.x % THREADS;
+    if (V > 1 && p < pixels) f(Loose<T, 1>{{x[p]}}, p);
 }
 
-template <int THREADS, typename P, typename F>
-__device__ __forceinline__ void each_pack_of_two(const P* x, const P* y, int packs, F f)
+template <int THREADS, int V, typename T, typename F>
+__device__ __forceinline__ void each_pack_of_two(const T* x, const T* y, int pixels, F f)
 {
-    int p = threadIdx.x % THREADS;
-    for (; p + (kAhead - 1) * THREADS < packs; p += kAhead * THREADS) {
+    using P = Loose<T, V>;
+    int p = threadIdx.x % THREADS * V;
+    for (; p + (kAhead - 1) * THREADS * V + V <= pixels; p += kAhead * THREADS * V) {
         P v[kAhead], w[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            v[u] = x[p + u * THREADS];
-            w[u] = y[p + u * THREADS];
+            __builtin_memcpy(&v[u], x + p + u * THREADS * V, sizeof(P));
+            __builtin_memcpy(&w[u], y + p + u * THREADS * V, sizeof(P));
         }
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) f(v[u], w[u], p + u * THREADS);
+        for (int u = 0; u < kAhead; ++u) f(v[u], w[u], p + u * THREADS * V);
     }
-    for (; p < packs; p += THREADS) f(x[p], y[p], p);
+    for (; p + V <= pixels; p += THREADS * V) {
+        P v, w;
+        __builtin_memcpy(&v, x + p, sizeof(P));
+        __builtin_memcpy(&w, y + p, sizeof(P));
+        f(v, w, p);
+    }
+    p = pixels / V * V + threadIdx.x % THREADS;
+    if (V > 1 && p < pixels) f(Loose<T, 1>{{x[p]}}, Loose<T, 1>{{y[p]}}, p);
+}
+
+// stream_out to anywhere.
+template <typename T, int V>
+__device__ __forceinline__ void stream_loose(T* to, const Loose<T, V>& v)
+{
+    if constexpr (sizeof(T) * V == 16) {
+        typedef uint32_t quad __attribute__((ext_vector_type(4)));
+        typedef quad loose_quad __attribute__((aligned(2)));
+        __builtin_nontemporal_store(__builtin_bit_cast(quad, v), reinterpret_cast<loose_quad*>(to));
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) to[j] = v.v[j];
+    }
 }
 
 template <int THREADS, typename A>
@@ -783,18 +820,15 @@ __global__ void __launch_bounds__(kT) gn_first_moments(const T* __restrict__ x, 
     const long plane = plane_of<THREADS>();
     if (plane >= g.planes) return;
     const T* base = x + plane * g.pixels;
-    const Pack<T, V>* packs = reinterpret_cast<const Pack<T, V>*>(base);
     const A first = (A)base[0];
     A s1 = (A)0;
-    each_pack<THREADS>(packs, g.pixels / V, [&](const Pack<T, V>& v, int) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) s1 += (A)v.v[j] - first;
+    each_pack<THREADS, V>(base, g.pixels, [&](const auto& v, int) {
+        for (const T& e : v.v) s1 += (A)e - first;
     });
     const A mean = first + plane_sum<THREADS>(s1, part) / (A)g.pixels;
     A s2 = (A)0;
-    each_pack<THREADS>(packs, g.pixels / V, [&](const Pack<T, V>& v, int) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) s2 += ((A)v.v[j] - mean) * ((A)v.v[j] - mean);
+    each_pack<THREADS, V>(base, g.pixels, [&](const auto& v, int) {
+        for (const T& e : v.v) s2 += ((A)e - mean) * ((A)e - mean);
     });
     s2 = plane_sum<THREADS>(s2, part);
     if (threadIdx.x % THREADS == 0) partial[plane] = Moments<A>{mean, s2};
@@ -820,13 +854,11 @@ __global__ void __launch_bounds__(kT) gn_first_apply(const T* __restrict__ x, co
         inv_std_out[group] = inv_std;
     }
     const A scale = inv_std * gamma[c], shift = beta[c];
-    Pack<T, V>* out = reinterpret_cast<Pack<T, V>*>(y + plane * g.pixels);
-    each_pack<THREADS>(reinterpret_cast<const Pack<T, V>*>(x + plane * g.pixels), g.pixels / V,
-                       [&](Pack<T, V> v, int p) {
-#pragma unroll
-                           for (int j = 0; j < V; ++j) v.v[j] = (T)act<ACT>(((A)v.v[j] - mean) * scale + shift);
-                           stream_out(out + p, v);
-                       });
+    T* out = y + plane * g.pixels;
+    each_pack<THREADS, V>(x + plane * g.pixels, g.pixels, [&](auto v, int p) {
+        for (T& e : v.v) e = (T)act<ACT>(((A)e - mean) * scale + shift);
+        stream_loose(out + p, v);
+    });
 }
 
 // A workgroup holds a group: x is read once.  `join` makes one group of all threads for join_threads.
@@ -901,17 +933,16 @@ __global__ void __launch_bounds__(kT) gn_first_bwd_sums(const T* __restrict__ dy
     const int c = (int)(plane % g.channels);
     const ChanBwd<A> ch = chan_bwd<ACT>(mean[plane / g.cg], inv_std[plane / g.cg], gamma[c], beta[c]);
     A s1 = (A)0, s2 = (A)0;
-    each_pack_of_two<THREADS>(reinterpret_cast<const Pack<T, V>*>(x + plane * g.pixels),
-                              reinterpret_cast<const Pack<T, V>*>(dy + plane * g.pixels), g.pixels / V,
-                              [&](const Pack<T, V>& xv, const Pack<T, V>& dv, int) {
+    auto add = [&](const auto& xv, const auto& dv, int) {
 #pragma unroll
-                                  for (int j = 0; j < V; ++j) {
-                                      const A xn = ((A)xv.v[j] - ch.mean) * ch.inv_std;
-                                      const A dz = dz_of<ACT>(ch, (A)xv.v[j], xn, (A)dv.v[j]);
-                                      s1 += dz;
-                                      s2 += dz * xn;
-                                  }
-                              });
+        for (unsigned j = 0; j < sizeof(xv) / sizeof(T); ++j) {
+            const A xn = ((A)xv.v[j] - ch.mean) * ch.inv_std;
+            const A dz = dz_of<ACT>(ch, (A)xv.v[j], xn, (A)dv.v[j]);
+            s1 += dz;
+            s2 += dz * xn;
+        }
+    };
+    each_pack_of_two<THREADS, V>(x + plane * g.pixels, dy + plane * g.pixels, g.pixels, add);
     s1 = plane_sum<THREADS>(s1, part);
     s2 = plane_sum<THREADS>(s2, part);
     if (threadIdx.x % THREADS == 0) {
@@ -935,18 +966,16 @@ __global__ void __launch_bounds__(kT) gn_first_bwd_apply(const T* __restrict__ d
     const long group = plane / g.cg;
     const ChanBwd<A> ch = chan_bwd<ACT>(mean[group], inv_std[group], gamma[c], beta[c]);
     const A a = ab[2 * group], b = ab[2 * group + 1];
-    Pack<T, V>* out = reinterpret_cast<Pack<T, V>*>(dx + plane * g.pixels);
-    each_pack_of_two<THREADS>(reinterpret_cast<const Pack<T, V>*>(x + plane * g.pixels),
-                              reinterpret_cast<const Pack<T, V>*>(dy + plane * g.pixels), g.pixels / V,
-                              [&](const Pack<T, V>& xv, Pack<T, V> dv, int p) {
+    T* out = dx + plane * g.pixels;
+    each_pack_of_two<THREADS, V>(x + plane * g.pixels, dy + plane * g.pixels, g.pixels, [&](const auto& xv, auto dv, int p) {
 #pragma unroll
-                                  for (int j = 0; j < V; ++j) {
-                                      const A xn = ((A)xv.v[j] - ch.mean) * ch.inv_std;
-                                      const A dz = dz_of<ACT>(ch, (A)xv.v[j], xn, (A)dv.v[j]);
-                                      dv.v[j] = (T)dx_of(ch, xn, dz, a, b);
-                                  }
-                                  stream_out(out + p, dv);
-                              });
+        for (unsigned j = 0; j < sizeof(xv) / sizeof(T); ++j) {
+            const A xn = ((A)xv.v[j] - ch.mean) * ch.inv_std;
+            const A dz = dz_of<ACT>(ch, (A)xv.v[j], xn, (A)dv.v[j]);
+            dv.v[j] = (T)dx_of(ch, xn, dz, a, b);
+        }
+        stream_loose(out + p, dv);
+    });
 }
 
 // A and B of each group: one wave a group.
@@ -1177,21 +1206,16 @@ int with_pack(int v, F f)
 
 bool too_many(long blocks) { return blocks * kT >= (1l << 32); }      // a launch counts its threads in 32 bits
 
-// Calls launch(elements of a pack, threads of a plane) for channels first: eight packs or more to a thread, where a plane has
-// them, so that small planes share workgroups.
+// Calls launch(threads of a plane) for channels first: eight packs or more to a thread, where a plane has them, so that small
+// planes share workgroups.
 template <typename T, typename F>
-int with_plane(int pixels, bool aligned, F launch)
+int with_plane(int pixels, F launch)
 {
     using std::integral_constant;
-    constexpr int V = 16 / sizeof(T);
-    auto threads = [&](auto v) {
-        const int packs = pixels / decltype(v)::value;
-        if (packs < 16 * 8) return launch(v, integral_constant<int, 16>());
-        if (packs < kWave * 8) return launch(v, integral_constant<int, kWave>());
-        return launch(v, integral_constant<int, kT>());
-    };
-    if (aligned && pixels % V == 0) return threads(integral_constant<int, V>());
-    return threads(integral_constant<int, 1>());
+    const int packs = pixels / (16 / (int)sizeof(T));
+    if (packs < 16 * 8) return launch(integral_constant<int, 16>());
+    if (packs < kWave * 8) return launch(integral_constant<int, kWave>());
+    return launch(integral_constant<int, kT>());
 }
 
 long plane_blocks(long planes, int threads) { return (planes + kT / threads - 1) / (kT / threads); }
@@ -1244,8 +1268,8 @@ int forward(int nhwc, const T* x, const wide_t<T>* gamma, const wide_t<T>* beta,
         HIP_RETURN_IF_LAUNCH_FAILED();
         return PYDTNN_HIP_OK;
     }
-    return with_plane<T>(pixels, aligned, [&](auto pack, auto threads) {
-        constexpr int V = decltype(pack)::value, N = decltype(threads)::value;
+    return with_plane<T>(pixels, [&](auto threads) {
+        constexpr int V = 16 / sizeof(T), N = decltype(threads)::value;
         const long blocks = plane_blocks(g.planes, N);
         if (too_many(blocks)) return PYDTNN_HIP_ERR_UNSUPPORTED;
         hipLaunchKernelGGL((gn_first_moments<T, V, N>), dim3((unsigned)blocks), dim3(kT), 0, st, x, part, g);
@@ -1300,8 +1324,8 @@ int backward(int nhwc, const T* dy, const T* x, const wide_t<T>* gamma, const wi
         });
     }
     const GnFirst g = {images * channels, pixels, channels, cg, make_fastdiv((uint32_t)pixels)};
-    return with_plane<T>(pixels, aligned16(x) && aligned16(dy) && aligned16(dx), [&](auto pack, auto threads) {
-        constexpr int V = decltype(pack)::value, N = decltype(threads)::value;
+    return with_plane<T>(pixels, [&](auto threads) {
+        constexpr int V = 16 / sizeof(T), N = decltype(threads)::value;
         const long blocks = plane_blocks(g.planes, N);
         if (too_many(blocks)) return PYDTNN_HIP_ERR_UNSUPPORTED;
         A* ab = sums + 2 * g.planes;
