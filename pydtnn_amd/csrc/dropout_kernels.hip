@@ -34,7 +34,7 @@ __device__ __forceinline__ uint4 philox(uint64_t call, uint64_t offset, uint64_t
     return make_uint4(c0, c1, c2, c3);
 }
 
-template <typename T, bool PACKED>
+template <typename T>
 __global__ void __launch_bounds__(kT) dropout_kernel(const T* x, T* y, long total, uint32_t threshold, wide_t<T> scale,
                                                      uint64_t seed, uint64_t offset, const int64_t* offset_dev)
 {
@@ -48,11 +48,12 @@ __global__ void __launch_bounds__(kT) dropout_kernel(const T* x, T* y, long tota
         const uint32_t u = (j & 1) ? word[j / 2] >> 16 : word[j / 2] & 0xffffu;
         return u >= threshold ? (T)((wide_t<T>)v * scale) : (T)0.0f;
     };
-    if (PACKED && first + kPerCall <= total) {
-        Pack<T, kPerCall> p = *reinterpret_cast<const Pack<T, kPerCall>*>(x + first);
+    if (first + kPerCall <= total) {      // accesses of 16 bytes, wherever the tensors start
+        T p[kPerCall];
+        __builtin_memcpy(p, x + first, sizeof(p));
 #pragma unroll
-        for (int j = 0; j < kPerCall; ++j) p.v[j] = one(j, p.v[j]);
-        *reinterpret_cast<Pack<T, kPerCall>*>(y + first) = p;
+        for (int j = 0; j < kPerCall; ++j) p[j] = one(j, p[j]);
+        __builtin_memcpy(y + first, p, sizeof(p));
     } else {
 #pragma unroll
         for (int j = 0; j < kPerCall; ++j)
@@ -75,12 +76,8 @@ int pydtnn_hip_dropout(int dtype, const void* x, void* y, long total, double rat
     const hipStream_t st = convint::as_stream(stream);
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        if (aligned16(x) && aligned16(y))
-            hipLaunchKernelGGL((dropout_kernel<T, true>), dim3((unsigned)blocks), dim3(kT), 0, st, (const T*)x, (T*)y,
-                               total, threshold, (wide_t<T>)scale, seed, offset, offset_dev);
-        else
-            hipLaunchKernelGGL((dropout_kernel<T, false>), dim3((unsigned)blocks), dim3(kT), 0, st, (const T*)x, (T*)y,
-                               total, threshold, (wide_t<T>)scale, seed, offset, offset_dev);
+        hipLaunchKernelGGL((dropout_kernel<T>), dim3((unsigned)blocks), dim3(kT), 0, st, (const T*)x, (T*)y, total, threshold,
+                           (wide_t<T>)scale, seed, offset, offset_dev);
         HIP_RETURN_IF_LAUNCH_FAILED();
         return PYDTNN_HIP_OK;
     });
