@@ -110,6 +110,17 @@ def test_group_norm(ops, shape, dtype, nhwc):
         check_gn(ops, *gn_inputs(shape, dtype, nhwc, 5), activation, nhwc)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [(1, (225, 223), 6, 2), (2, (47, 43), 5, 1), (3, (13, 11), 7, 7), (2, (3, 1), 6, 3)], ids=str)
+def test_group_norm_of_planes_of_odd_extents(ops, shape, dtype):
+    """Planes and groups that no pack divides and that start off the boundaries of packs, of sizes for a workgroup, a wave and
+    a part of one; forward in two passes."""
+    announce("group norm, odd planes", shape, dtype)
+    x, dy, gamma, beta, groups = gn_inputs(shape, dtype, False, 7)
+    check_gn(ops, x, dy, gamma, beta, groups, "relu", False)
+    check_gn(ops, misaligned(x), misaligned(dy), gamma, beta, groups, "silu", False)
+
+
 @pytest.mark.parametrize("nhwc", [True, False], ids=["last", "first"])
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("shape", [(64, (13, 17), 128, 8), (64, (23, 23), 128, 4), (30, (18, 17), 544, 17)], ids=str)
