@@ -898,21 +898,22 @@ __global__ void __launch_bounds__(THREADS) gn_first_whole(const T* __restrict__ 
     });
     __syncthreads();
     const A mu = mean, r = inv_std;
-    const bool one = g.pixels % V == 0;      // whether a pack is of one channel
+    const bool one = g.pixels % V == 0;      // whether each pack is of one channel
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
         const int p = threadIdx.x + i * THREADS;
         if (p >= packs) continue;
-        int c = c0 + (int)fd_div((uint32_t)(p * V), g.by_pixels);
-        A scale = r * gamma[c], shift = beta[c];
+        const uint32_t k = fd_div((uint32_t)(p * V), g.by_pixels);
+        if (one || k == fd_div((uint32_t)(p * V + V - 1), g.by_pixels)) {
+            const A scale = r * gamma[c0 + k], shift = beta[c0 + k];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            if (!one && j > 0) {
-                c = c0 + (int)fd_div((uint32_t)(p * V + j), g.by_pixels);
-                scale = r * gamma[c];
-                shift = beta[c];
+            for (int j = 0; j < V; ++j) v[i].v[j] = (T)act<ACT>(((A)v[i].v[j] - mu) * scale + shift);
+        } else {      // a pack that straddles channels
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const int c = c0 + (int)fd_div((uint32_t)(p * V + j), g.by_pixels);
+                v[i].v[j] = (T)act<ACT>(((A)v[i].v[j] - mu) * (r * gamma[c]) + beta[c]);
             }
-            v[i].v[j] = (T)act<ACT>(((A)v[i].v[j] - mu) * scale + shift);
         }
         out[p] = v[i];
     }
