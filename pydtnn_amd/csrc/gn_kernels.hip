@@ -748,8 +748,7 @@ __device__ __forceinline__ void each_pack(const T* x, int pixels, F f)
         __builtin_memcpy(&v, x + p, sizeof(P));
         f(v, p);
     }
-    p = pixels / V * V + threadIdx.x % THREADS;
-    if (V > 1 && p < pixels) f(Loose<T, 1>{{x[p]}}, p);
+    for (p = pixels / V * V + threadIdx.x % THREADS; p < pixels; p += THREADS) f(Loose<T, 1>{{x[p]}}, p);
 }
 
 template <int THREADS, int V, typename T, typename F>
@@ -773,8 +772,8 @@ __device__ __forceinline__ void each_pack_of_two(const T* x, const T* y, int pix
         __builtin_memcpy(&w, y + p, sizeof(P));
         f(v, w, p);
     }
-    p = pixels / V * V + threadIdx.x % THREADS;
-    if (V > 1 && p < pixels) f(Loose<T, 1>{{x[p]}}, Loose<T, 1>{{y[p]}}, p);
+    for (p = pixels / V * V + threadIdx.x % THREADS; p < pixels; p += THREADS)
+        f(Loose<T, 1>{{x[p]}}, Loose<T, 1>{{y[p]}}, p);
 }
 
 // stream_out to anywhere.
@@ -1208,12 +1207,15 @@ int with_pack(int v, F f)
 bool too_many(long blocks) { return blocks * kT >= (1l << 32); }      // a launch counts its threads in 32 bits
 
 // Calls launch(threads of a plane) for channels first: eight packs or more to a thread, where a plane has them, so that small
-// planes share workgroups.
+// planes share workgroups; four threads for the smallest, whose time goes into a plane's constants and sums (backward
+// 64 x 1024 x 4 x 4 in float32: 13 us with four, 19 with sixteen; 64 x 2048 x 7 x 7, of twelve packs: 47 and 37, and of six in
+// bfloat16: 29 and 36).
 template <typename T, typename F>
 int with_plane(int pixels, F launch)
 {
     using std::integral_constant;
     const int packs = pixels / (16 / (int)sizeof(T));
+    if (packs <= 4 * 2) return launch(integral_constant<int, 4>());
     if (packs < 16 * 8) return launch(integral_constant<int, 16>());
     if (packs < kWave * 8) return launch(integral_constant<int, kWave>());
     return launch(integral_constant<int, kT>());
