@@ -484,9 +484,16 @@ int pydtnn_hip_dropout(int dtype, const void *x, void *y, long total, double rat
  *       nearest e4m3 value, to even between two.  A block that holds an infinity or a NaN is NaN throughout, its scale 1.
  *   pydtnn_hip_matmul_fp8: y (m, n) = relu?( dequantised(quantised(x)) * dequantised(w)^T + bias ) with x (m, k) quantised on
  *       the way and wq (n, kp), wscales as pydtnn_hip_quantize_fp8 makes them of the (n, k) weights, once.  bias (n) is
- *       float32 or NULL; sums are held in float32.
+ *       float32 or NULL.
+ *       Sums with float32 x: in float32, 24 bits of every product and sum.  With float16 or bfloat16 x the products of each
+ *       eight consecutive k (from a multiple of 8) are first cut off 13 bits below the largest of the eight, towards zero;
+ *       the eights are then added in float32.  A result is off by up to 7 * 2^-13 of the largest product of each eight: as a
+ *       rule 1e-5 of it, a fortieth of the half step that float16 rounds by, but more of a result that is small because large
+ *       products of it cancel.  Where that matters, hand x over as float32.
  * x and y are float32, float16 or bfloat16 (`dtype`; PYDTNN_HIP_ERR_INVALID for float64).  q and the workspace are aligned to
- * 16 bytes, scales to 4.  m and n are at most 2^30, k at most 2^23.  For float32 results the dequantised values go through
+ * 16 bytes, scales to 4.  m and n are at most 2^30, k at most 2^23, and a launch has fewer than 2^32 threads
+ * (PYDTNN_HIP_ERR_UNSUPPORTED): rows * words is at most 2^26 - 4 where rows are quantised, in a product of more than 16 rows too,
+ * and n under 2^27 in one of up to 16.  For float32 results the dequantised values go through
  * bfloat16: those of 2^128 are infinite, and those under 2^-126 may count as 0.  Workspace:
  * pydtnn_hip_matmul_fp8_workspace_bytes(dtype, m, n, k). */
 int pydtnn_hip_quantize_fp8(int dtype, const void *x, long rows, long k, uint8_t *q, uint8_t *scales, void *stream);

@@ -691,3 +691,29 @@ def test_builders_with_group_norm_and_seeded_dropout(pd):
     for layer in model.get_all_layers():
         if type(layer).__name__ == "GroupNormalization":
             assert torch.isfinite(layer.dgamma).all() and layer.dgamma.abs().max() > 0
+
+
+# --------------------------------------------------------------------------- sums of the e4m3 product
+@pytest.mark.parametrize("m", [2, 40])
+@pytest.mark.parametrize("dtype", FP8_DTYPES, ids=str)
+def test_matmul_fp8_adds_what_its_documentation_says(ops, m, dtype):
+    """Two eights whose largest products, 2^16 and -2^16, cancel and leave seven products of 2^3 and seven of 2^2: the former
+    are 13 bits below the largest, the latter 14.  In 24 bits the sum is 84; for 16-bit types it is off by at most 7 * 2^-13 of
+    the largest product of each eight, which is what the test's bound is of."""
+    announce("matmul_fp8 cancelling", m, dtype)
+    row = torch.zeros(128)
+    row[0], row[8] = 256.0, -256.0
+    row[1:8], row[9:16] = 2.0, 1.0
+    weights = torch.zeros(128)
+    weights[0] = weights[8] = 256.0
+    weights[1:8] = weights[9:16] = 4.0
+    x = row.repeat(m, 1).to(dtype).cuda()
+    wq, ws = ops.quantize_fp8(weights.repeat(20, 1).cuda())
+    y = oo.host64(ops.matmul_fp8(x, wq, ws))
+    if dtype == torch.float32:
+        assert np.all(y == 84.0)
+    else:
+        assert np.all(np.abs(y - 84.0) <= 2 * 7 * 2.0 ** -13 * 2.0 ** 16)
+        assert torch.all(ops.matmul_fp8(x.float(), wq, ws) == 84.0)
+    ref, bound = oo.matmul_fp8(oo.host64(x), *oo.quantize_fp8(oo.host64(weights.repeat(20, 1))), None, False, dtype)
+    assert np.all(ref == 84.0) and np.all(np.abs(y - ref) <= bound)

@@ -228,3 +228,13 @@ def test_a_float64_model_has_no_8_bit_layers():
         pd.Model(dtype="float64", enable_fp8_fc=True)
     with pytest.raises(ValueError):
         pd.Model(dtype="float64").apply_layer_fusion(fp8_fc=True)
+
+
+def test_fp8_refuses_launches_of_too_many_threads(lib):
+    """A wave to each word of four blocks: 2^26 of them would be 2^32 threads."""
+    p = ctypes.c_void_p(FAKE)
+    for rows, k in ((1 << 26, 128), (1 << 24, 2048), ((1 << 26) - 3, 1)):
+        assert lib.pydtnn_hip_quantize_fp8(0, p, rows, k, p, p, None) == 4
+        need = lib.pydtnn_hip_matmul_fp8_workspace_bytes(0, rows, 8, k)
+        assert lib.pydtnn_hip_matmul_fp8(0, p, rows, k, p, p, 8, None, 0, p, p, need, None) == 4
+    assert lib.pydtnn_hip_matmul_fp8(0, p, 1, 128, p, p, 1 << 27, None, 0, p, None, 0, None) == 4
