@@ -519,12 +519,15 @@ def conv_i2c_dx(nhwc, geom13, weights, dy, dx):
 def _on_its_device(f):
     """Runs ``f`` with the device of its first argument as the current one, so that the work goes to that device's
     current stream."""
+    first = f.__code__.co_varnames[0]
+
     @functools.wraps(f)
-    def g(x, *args, **kwargs):
-        if x.is_cuda and x.device.index != torch.cuda.current_device():
+    def g(*args, **kwargs):
+        x = args[0] if args else kwargs.get(first)
+        if x is not None and x.is_cuda and x.device.index != torch.cuda.current_device():
             with torch.cuda.device(x.device):
-                return f(x, *args, **kwargs)
-        return f(x, *args, **kwargs)
+                return f(*args, **kwargs)
+        return f(*args, **kwargs)
     return g
 
 

@@ -1,6 +1,7 @@
 """CPU-side checks of the operators for several element types: the oracles against published values and differences, and
 what the entry points refuse (nothing here launches a kernel)."""
 import ctypes
+import inspect
 import os
 
 import numpy as np
@@ -238,3 +239,23 @@ def test_fp8_refuses_launches_of_too_many_threads(lib):
         need = lib.pydtnn_hip_matmul_fp8_workspace_bytes(0, rows, 8, k)
         assert lib.pydtnn_hip_matmul_fp8(0, p, rows, k, p, p, 8, None, 0, p, p, need, None) == 4
     assert lib.pydtnn_hip_matmul_fp8(0, p, 1, 128, p, p, 1 << 27, None, 0, p, None, 0, None) == 4
+
+
+@pytest.mark.parametrize("call", ["gn_forward", "gn_backward", "dropout", "dropout_backward", "quantize_fp8", "matmul_fp8"])
+def test_operators_take_their_arguments_by_name(ops, call):
+    """Each argument by the name that the signature gives it, the first of them positional or not: the calls get as far as the
+    refusal of tensors that are not on the GPU."""
+    x, v, s = torch.ones(2, 3, 3, 8), torch.ones(8), torch.ones(2, 4)
+    q, scales = torch.ones(6, 256).to(torch.float8_e4m3fn), torch.ones(6, 4, dtype=torch.uint8)
+    kwargs = {"gn_forward": dict(x=x, gamma=v, beta=v, groups=4, eps=1e-5, activation="relu", nhwc=True),
+              "gn_backward": dict(dy=x, x=x, gamma=v, beta=v, mean=s, inv_std=s, groups=4, activation="", nhwc=True, need_dx=True),
+              "dropout": dict(x=x, rate=0.5, seed=1, offset=2),
+              "dropout_backward": dict(dy=x, rate=0.5, seed=1, offset=2),
+              "quantize_fp8": dict(x=torch.ones(3, 200)),
+              "matmul_fp8": dict(x=torch.ones(3, 200), wq=q, wscales=scales, bias=None, relu=True)}[call]
+    assert list(inspect.signature(getattr(ops, call)).parameters) == list(kwargs)
+    with pytest.raises(ValueError, match="on the GPU"):
+        getattr(ops, call)(**kwargs)
+    with pytest.raises(ValueError, match="on the GPU"):
+        first = next(iter(kwargs))
+        getattr(ops, call)(kwargs.pop(first), **kwargs)
