@@ -10,6 +10,8 @@ pydtnn/backends/cpu/layers/conv_2d_cpu.py:89-143 does and installs it as ``self.
 ``self.backward``, so the fusion pass in ``model.py`` can test ``forward.__name__`` the way the
 reference does.
 """
+import operator
+
 import numpy as np
 import torch
 
@@ -670,8 +672,10 @@ class Dropout(Layer):
     def __init__(self, rate=0.5, seed=None):
         super().__init__()
         self.rate = min(1., max(0., rate))
-        if seed is not None and not 0 <= seed < 1 << 32:
-            raise ValueError("the seed of a Dropout layer is a number of 32 bits")
+        if seed is not None:
+            seed = operator.index(seed)
+            if not 0 <= seed < 1 << 32:
+                raise ValueError("the seed of a Dropout layer is a number of 32 bits")
         self.seed = seed
         self.mask = None
         self.step = None

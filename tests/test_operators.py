@@ -259,3 +259,15 @@ def test_operators_take_their_arguments_by_name(ops, call):
     with pytest.raises(ValueError, match="on the GPU"):
         first = next(iter(kwargs))
         getattr(ops, call)(kwargs.pop(first), **kwargs)
+
+
+@pytest.mark.parametrize("seed", [5, np.int32(5), np.uint32(5), np.uint64(5), np.int64(5)], ids=lambda v: type(v).__name__)
+def test_a_dropout_layers_seed_may_be_any_whole_number(seed):
+    """The layer's key is seed + (id << 32), which no type of 32 bits holds."""
+    import pydtnn_amd as pd
+    layer = pd.Dropout(rate=0.5, seed=seed)
+    layer.id = 3
+    assert layer._key() == 5 + (3 << 32) and type(layer._key()) is int
+    for bad in (1.5, "5", np.float32(5)):
+        with pytest.raises(TypeError):
+            pd.Dropout(rate=0.5, seed=bad)
