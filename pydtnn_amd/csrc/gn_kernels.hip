@@ -312,6 +312,25 @@ struct ChanFwd {
     }
 };
 
+// The same for every group by a kernel of its own, a wave a group, for passes whose workgroups would each join too much again.
+// A group is `units` of `unit` elements, in pieces of `run` units.
+template <typename A>
+__global__ void __launch_bounds__(kT) gn_join_groups(const Moments<A>* __restrict__ partial, A* __restrict__ mean_out,
+                                                     A* __restrict__ inv_std_out, long groups, int pieces, long units, long run,
+                                                     int unit, double eps)
+{
+    const long group = (long)blockIdx.x * kWaves + threadIdx.x / kWave;
+    if (group >= groups) return;
+    A mean, inv_std;
+    join_moments<A>(partial + group * pieces, pieces, [&](int i) { return (double)min(run, units - i * run) * unit; },
+                    (double)units * unit, eps, kWave, &mean, &inv_std);
+    if (threadIdx.x % kWave == 0) {
+        mean_out[group] = mean;
+        inv_std_out[group] = inv_std;
+    }
+}
+
+// Without `partial`, mean and inv_std hold the groups' statistics already.
 template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(kT) gn_last_apply(const T* __restrict__ x, const wide_t<T>* __restrict__ gamma,
                                                     const wide_t<T>* __restrict__ beta,
@@ -324,8 +343,15 @@ __global__ void __launch_bounds__(kT) gn_last_apply(const T* __restrict__ x, con
     const unsigned piece = piece_from_the_end(blockIdx.x, gridDim.x);
     if (piece >= g.pieces) return;
     const Place at = place_of(g, piece);
-    for (int k = threadIdx.x / g.group_lanes; k < g.slab_groups; k += kT / g.group_lanes) {
-        const long group = at.image * g.groups + at.slab * g.slab_groups + k;
+    const long first_group = at.image * g.groups + at.slab * g.slab_groups;
+    if (!partial) {
+        for (int k = threadIdx.x; k < g.slab_groups; k += kT) {
+            mean[k] = mean_out[first_group + k];
+            inv_std[k] = inv_std_out[first_group + k];
+        }
+    }
+    for (int k = threadIdx.x / g.group_lanes; partial && k < g.slab_groups; k += kT / g.group_lanes) {
+        const long group = first_group + k;
         A m, r;
         join_moments<A>(partial + group * g.splits, g.splits,
                         [&](int i) { return (double)(min(g.run, g.pixels - i * g.run)) * g.cg; },
@@ -547,8 +573,8 @@ __global__ void __launch_bounds__(kT) gn_last_bwd_sums(const T* __restrict__ dy,
 constexpr int kParamChannels = 4, kParamRows = kT / kParamChannels;
 
 template <typename A>
-__device__ __forceinline__ void bwd_params(const A* __restrict__ sums, A* __restrict__ dgamma, A* __restrict__ dbeta,
-                                           long pieces, int channels, int block)
+__device__ __forceinline__ void bwd_params(const A* __restrict__ s1, const A* __restrict__ s2, A* __restrict__ dgamma,
+                                           A* __restrict__ dbeta, long pieces, int channels, int block)
 {
     __shared__ double part1[kT], part2[kT];
     const int c = block * kParamChannels + threadIdx.x % kParamChannels, r = threadIdx.x / kParamChannels;
@@ -556,8 +582,8 @@ __device__ __forceinline__ void bwd_params(const A* __restrict__ sums, A* __rest
     if (c < channels) {
 #pragma unroll 4
         for (long i = r; i < pieces; i += kParamRows) {
-            t1 += (double)sums[i * channels + c];
-            t2 += (double)sums[(pieces + i) * channels + c];
+            t1 += (double)s1[i * channels + c];
+            t2 += (double)s2[i * channels + c];
         }
     }
     part1[threadIdx.x] = t1;
@@ -580,7 +606,19 @@ template <typename A>
 __global__ void __launch_bounds__(kT) gn_bwd_params(const A* __restrict__ sums, A* __restrict__ dgamma,
                                                     A* __restrict__ dbeta, long pieces, int channels)
 {
-    bwd_params(sums, dgamma, dbeta, pieces, channels, blockIdx.x);
+    bwd_params(sums, sums + pieces * channels, dgamma, dbeta, pieces, channels, blockIdx.x);
+}
+
+// The channel sums of each image from those of its runs, `blocks` workgroups an image: image_sums[image * channels + channel],
+// then the same of dz xn.
+template <typename A>
+__global__ void __launch_bounds__(kT) gn_bwd_images(const A* __restrict__ sums, A* __restrict__ image_sums, long images,
+                                                    int splits, int channels, int blocks)
+{
+    const long image = blockIdx.x / blocks;
+    const A* s1 = sums + image * splits * channels;
+    A* out = image_sums + image * channels;
+    bwd_params(s1, s1 + images * splits * channels, out + images * channels, out, splits, channels, blockIdx.x % blocks);
 }
 
 // A and B of one group from the channel sums of its runs, by `lanes` consecutive threads.
@@ -606,30 +644,39 @@ __device__ __forceinline__ void group_ab(const A* s1, const A* s2, const A* gamm
     }
 }
 
-// dx, and in the first workgroups dgamma and dbeta.
+// dx, and in the first workgroups dgamma and dbeta.  `ab`, unless it is null, holds A and B of each group.
 template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(kT) gn_last_bwd_apply(const T* __restrict__ dy, const T* __restrict__ x,
                                                         const wide_t<T>* __restrict__ gamma,
                                                         const wide_t<T>* __restrict__ beta,
                                                         const wide_t<T>* __restrict__ mean,
                                                         const wide_t<T>* __restrict__ inv_std,
-                                                        const wide_t<T>* __restrict__ sums, wide_t<T>* __restrict__ dgamma,
+                                                        const wide_t<T>* __restrict__ sums,
+                                                        const wide_t<T>* __restrict__ ab, wide_t<T>* __restrict__ dgamma,
                                                         wide_t<T>* __restrict__ dbeta, T* __restrict__ dx, int param_blocks,
                                                         GnLast g)
 {
     using A = wide_t<T>;
     __shared__ A group_a[kT * V], group_b[kT * V];
+    const A* sums2 = sums + g.images * g.splits * g.channels;
     if ((int)blockIdx.x < param_blocks) {
         if ((int)blockIdx.x * kParamChannels < g.channels)
-            bwd_params(sums, dgamma, dbeta, g.images * g.splits, g.channels, blockIdx.x);
+            bwd_params(sums, sums2, dgamma, dbeta, g.images * g.splits, g.channels, blockIdx.x);
         return;
     }
     const unsigned piece = piece_from_the_end(blockIdx.x - param_blocks, gridDim.x - param_blocks);
     if (piece >= g.pieces) return;
     const Place at = place_of(g, piece);
-    const A* s1 = sums + at.image * g.splits * g.channels;
-    for (int k = threadIdx.x / g.group_lanes; k < g.slab_groups; k += kT / g.group_lanes)
-        group_ab(s1, s1 + g.images * g.splits * g.channels, gamma, at.slab * g.width + k * g.cg, g.cg, g.splits, g.channels,
+    if (ab) {
+        const A* of_slab = ab + 2 * (at.image * g.groups + at.slab * g.slab_groups);
+        for (int k = threadIdx.x; k < g.slab_groups; k += kT) {
+            group_a[k] = of_slab[2 * k];
+            group_b[k] = of_slab[2 * k + 1];
+        }
+    }
+    const long from_run = at.image * g.splits * g.channels;
+    for (int k = threadIdx.x / g.group_lanes; !ab && k < g.slab_groups; k += kT / g.group_lanes)
+        group_ab(sums + from_run, sums2 + from_run, gamma, at.slab * g.width + k * g.cg, g.cg, g.splits, g.channels,
                  (double)g.cg * g.pixels, g.group_lanes, &group_a[k], &group_b[k]);
     __syncthreads();
     if (at.ty >= g.rows) return;
@@ -1048,6 +1095,25 @@ GnLast last_shape(long images, int channels, int pixels, int groups, int v)
     return g;
 }
 
+// Each workgroup of a second pass joins what the runs of its slab's groups left, which grows with the square of the runs: where
+// a lane would take more than kJoinForward moments, or kJoinBackward channel sums, a kernel (backward two) of a wave a
+// group joins them once.  In float32, groups of 8, 4 x 112 x 112 x 256 (191 runs): forward 24 a lane 31 us, joined once 27;
+// backward 191 a lane 54 and 47.  8 x 112 x 112 x 256 (96 runs): forward 12 a lane 48.8 and 48.5, backward 96 a lane 82.2 and
+// 81.9; 16 x 112 x 112 x 256 (48): forward 6 a lane 92.7 and 93.1, backward 48 a lane 174.6 and 176.3.  1 x 112 x 112 x 1024 (738
+// runs): forward in groups of one 2600 and 40, backward in groups of 16 600 and 58.
+constexpr long kJoinForward = 16, kJoinBackward = 64;
+
+// What a lane of a workgroup joins where each group has that many entries.
+long entries_of_lane(const GnLast& g, long entries)
+{
+    return ((long)g.slab_groups * g.group_lanes + kT - 1) / kT * ((entries + g.group_lanes - 1) / g.group_lanes);
+}
+
+bool joined_forward(const GnLast& g) { return entries_of_lane(g, g.splits) > kJoinForward; }
+
+// (a slab that is one run joins nothing twice)
+bool joined_backward(const GnLast& g) { return g.splits > 1 && entries_of_lane(g, g.cg) * g.splits > kJoinBackward; }
+
 // Where one kernel can hold a slab of an image in the registers of `threads` threads, `packs` packs of 16 bytes each (of x,
 // and in the backward pass as many of dy): the smallest slab of whole groups whose rows have at least `line` bytes, or all
 // channels; at most `most` of them.
@@ -1165,7 +1231,7 @@ size_t workspace_bytes_of(int dtype, bool nhwc, bool backward, long images, int 
 {
     const int size = size_of(dtype), wide = dtype == kDtypeF64 ? 8 : 4;
     const int v = aligned ? pack_of(size, channels, channels / groups) : 1;
-    long moments = images * channels, sums = images * channels;      // pieces of groups, of channels
+    long moments = images * channels, sums = images * channels, joined = 0;      // pieces of groups, of channels, channels of images
     if (nhwc) {
         auto fits = [&](int line, long most, auto threads, auto packs) {
             GnLast g;
@@ -1176,10 +1242,11 @@ size_t workspace_bytes_of(int dtype, bool nhwc, bool backward, long images, int 
         const GnLast g = last_shape(images, channels, pixels, groups, v);
         moments = images * groups * g.splits;
         sums = images * channels * g.splits;
+        if (joined_backward(g)) joined = images * channels;
     } else if (!backward && first_whole(size, pixels, channels / groups, aligned, images * groups)) {
         return 0;
     }
-    return (size_t)(backward ? 2 * sums + 2 * images * groups : 2 * moments) * wide;
+    return (size_t)(backward ? 2 * (sums + joined + images * groups) : 2 * moments) * wide;
 }
 
 template <typename F>
@@ -1221,6 +1288,8 @@ int with_plane(int pixels, F launch)
     return launch(integral_constant<int, kT>());
 }
 
+long wave_blocks(long waves) { return (waves + kWaves - 1) / kWaves; }
+
 long plane_blocks(long planes, int threads) { return (planes + kT / threads - 1) / (kT / threads); }
 
 unsigned eights(long blocks) { return (unsigned)((blocks + 7) / 8 * 8); }
@@ -1246,12 +1315,16 @@ int forward(int nhwc, const T* x, const wide_t<T>* gamma, const wide_t<T>* beta,
             return PYDTNN_HIP_OK;
         }
         g = last_shape(images, channels, pixels, groups, v);
-        if (too_many(g.pieces + 8)) return PYDTNN_HIP_ERR_UNSUPPORTED;
+        if (too_many(g.pieces + 8) || (joined_forward(g) && too_many(wave_blocks(images * groups))))
+            return PYDTNN_HIP_ERR_UNSUPPORTED;
         return with_pack(v, [&](auto pack) {
             constexpr int V = decltype(pack)::value * sizeof(T) <= 16 ? decltype(pack)::value : 1;
             hipLaunchKernelGGL((gn_last_moments<T, V>), dim3((unsigned)g.pieces), dim3(kT), 0, st, x, part, g);
-            hipLaunchKernelGGL((gn_last_apply<T, V, ACT>), dim3(eights(g.pieces)), dim3(kT), 0, st, x, gamma, beta, part, y,
-                               mean, inv_std, eps, g);
+            if (joined_forward(g))
+                hipLaunchKernelGGL((gn_join_groups<A>), dim3((unsigned)wave_blocks(images * groups)), dim3(kT), 0, st, part, mean,
+                                   inv_std, images * groups, g.splits, (long)pixels, (long)g.run, g.cg, eps);
+            hipLaunchKernelGGL((gn_last_apply<T, V, ACT>), dim3(eights(g.pieces)), dim3(kT), 0, st, x, gamma, beta,
+                               joined_forward(g) ? nullptr : part, y, mean, inv_std, eps, g);
             HIP_RETURN_IF_LAUNCH_FAILED();
             return PYDTNN_HIP_OK;
         });
@@ -1314,13 +1387,23 @@ int backward(int nhwc, const T* dy, const T* x, const wide_t<T>* gamma, const wi
         g = last_shape(images, channels, pixels, groups, v);
         // the first workgroups of the second pass, in eights so that its pieces keep their dies, are those of the parameters
         const long ahead = eights(param_blocks);
-        if (too_many(g.pieces + 8 + ahead)) return PYDTNN_HIP_ERR_UNSUPPORTED;
+        const bool joined = dx && joined_backward(g);
+        if (too_many(g.pieces + 8 + ahead) || (joined && too_many(images * std::max((long)param_blocks, wave_blocks(groups)))))
+            return PYDTNN_HIP_ERR_UNSUPPORTED;
+        A* image_sums = sums + 2 * images * g.splits * channels;
+        A* ab = joined ? image_sums + 2 * images * channels : nullptr;
         return with_pack(v, [&](auto pack) {
             constexpr int V = decltype(pack)::value * sizeof(T) <= 16 ? decltype(pack)::value : 1;
             hipLaunchKernelGGL((gn_last_bwd_sums<T, V, ACT>), dim3((unsigned)g.pieces), dim3(kT), 0, st, dy, x, gamma, beta,
                                mean, inv_std, sums, g);
+            if (joined) {
+                hipLaunchKernelGGL((gn_bwd_images<A>), dim3((unsigned)(images * param_blocks)), dim3(kT), 0, st, sums, image_sums,
+                                   images, g.splits, channels, param_blocks);
+                hipLaunchKernelGGL((gn_bwd_groups<A>), dim3((unsigned)wave_blocks(images * groups)), dim3(kT), 0, st, image_sums,
+                                   gamma, ab, images, channels, groups, (double)cg * pixels);
+            }
             if (dx) hipLaunchKernelGGL((gn_last_bwd_apply<T, V, ACT>), dim3((unsigned)(ahead + eights(g.pieces))), dim3(kT), 0,
-                                       st, dy, x, gamma, beta, mean, inv_std, sums, dgamma, dbeta, dx, (int)ahead, g);
+                                       st, dy, x, gamma, beta, mean, inv_std, sums, ab, dgamma, dbeta, dx, (int)ahead, g);
             else params(images * g.splits);
             HIP_RETURN_IF_LAUNCH_FAILED();
             return PYDTNN_HIP_OK;
@@ -1336,7 +1419,7 @@ int backward(int nhwc, const T* dy, const T* x, const wide_t<T>* gamma, const wi
                            inv_std, sums, g);
         params(images);
         if (dx) {
-            hipLaunchKernelGGL((gn_bwd_groups<A>), dim3((unsigned)((images * groups + kWaves - 1) / kWaves)), dim3(kT), 0, st,
+            hipLaunchKernelGGL((gn_bwd_groups<A>), dim3((unsigned)wave_blocks(images * groups)), dim3(kT), 0, st,
                                sums, gamma, ab, images, channels, groups, (double)cg * pixels);
             hipLaunchKernelGGL((gn_first_bwd_apply<T, V, N, ACT>), dim3((unsigned)blocks), dim3(kT), 0, st, dy, x, gamma, beta,
                                mean, inv_std, ab, dx, g);
@@ -1391,7 +1474,7 @@ int pydtnn_hip_gn_backward(int dtype, int nhwc, const void* dy, const void* x, c
     if (!workspace || !aligned16(workspace) || workspace_bytes < need) return PYDTNN_HIP_ERR_WORKSPACE;
     // (the kernels of channels and of groups; those of x count their own)
     if (too_many((channels + kParamChannels - 1) / kParamChannels) ||
-        (!nhwc && too_many((images * groups + kWaves - 1) / kWaves)))
+        (!nhwc && too_many(wave_blocks(images * groups))))
         return PYDTNN_HIP_ERR_UNSUPPORTED;
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);

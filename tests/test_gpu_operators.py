@@ -717,3 +717,45 @@ def test_matmul_fp8_adds_what_its_documentation_says(ops, m, dtype):
         assert torch.all(ops.matmul_fp8(x.float(), wq, ws) == 84.0)
     ref, bound = oo.matmul_fp8(oo.host64(x), *oo.quantize_fp8(oo.host64(weights.repeat(20, 1))), None, False, dtype)
     assert np.all(ref == 84.0) and np.all(np.abs(y - ref) <= bound)
+
+
+# --------------------------------------------------------------------------- group norm: few images of many runs
+def least_us(f):
+    """The least time of a call among calls, of five blocks of ten."""
+    f()
+    torch.cuda.synchronize()
+    times = []
+    for _ in range(5):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        for _ in range(10):
+            f()
+        end.record()
+        end.synchronize()
+        times.append(start.elapsed_time(end) * 100)
+    return min(times)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [(1, (90, 88), 520, 520), (1, (112, 112), 256, 1), (2, (61, 60), 512, 128), (1, (120, 121), 27, 9)],
+                         ids=str)
+def test_group_norm_of_few_images_of_many_runs(ops, shape, dtype):
+    """Images cut into hundreds of runs, whose sums kernels of their own join."""
+    announce("group norm, many runs", shape, dtype)
+    x, dy, gamma, beta, groups = gn_inputs(shape, dtype, True, 8)
+    check_gn(ops, x, dy, gamma, beta, groups, "silu", True)
+    check_gn(ops, misaligned(x), dy, gamma, beta, groups, "relu", True)
+
+
+@pytest.mark.parametrize("groups", [1, 16, 64, 256, 1024])
+def test_group_norm_of_one_large_image_costs_a_few_copies(ops, groups):
+    """What the second pass joins does not grow with the square of the runs: one image of 51 MB, cut into over 700 runs, takes
+    at most eight times what a copy of it takes in either direction (they move it three and five times)."""
+    announce("group norm, one image", groups)
+    x, dy, gamma, beta, _ = gn_inputs((1, (112, 112), 1024, groups), torch.float32, True, 9)
+    y, mean, inv_std = ops.gn_forward(x, gamma, beta, groups)
+    copy = least_us(x.clone)
+    forward = least_us(lambda: ops.gn_forward(x, gamma, beta, groups))
+    backward = least_us(lambda: ops.gn_backward(dy, x, gamma, beta, mean, inv_std, groups))
+    print(f"copy {copy:.1f} us, forward {forward:.1f}, backward {backward:.1f}")
+    assert forward < 8 * copy and backward < 8 * copy, (copy, forward, backward)
