@@ -880,6 +880,7 @@ __global__ void __launch_bounds__(kT) gn_first_moments(const T* __restrict__ x, 
     if (threadIdx.x % THREADS == 0) partial[plane] = Moments<A>{mean, s2};
 }
 
+// Without `partial`, mean and inv_std hold the groups' statistics already.
 template <typename T, int V, int THREADS, int ACT>
 __global__ void __launch_bounds__(kT) gn_first_apply(const T* __restrict__ x, const wide_t<T>* __restrict__ gamma,
                                                      const wide_t<T>* __restrict__ beta,
@@ -893,11 +894,16 @@ __global__ void __launch_bounds__(kT) gn_first_apply(const T* __restrict__ x, co
     const long group = plane / g.cg;
     const int c = (int)(plane % g.channels);
     A mean, inv_std;
-    join_moments<A>(partial + group * g.cg, g.cg, [&](int) { return (double)g.pixels; }, (double)g.pixels * g.cg, eps,
-                    THREADS < kWave ? THREADS : kWave, &mean, &inv_std);
-    if (plane % g.cg == 0 && threadIdx.x % THREADS == 0) {
-        mean_out[group] = mean;
-        inv_std_out[group] = inv_std;
+    if (!partial) {
+        mean = mean_out[group];
+        inv_std = inv_std_out[group];
+    } else {
+        join_moments<A>(partial + group * g.cg, g.cg, [&](int) { return (double)g.pixels; }, (double)g.pixels * g.cg, eps,
+                        THREADS < kWave ? THREADS : kWave, &mean, &inv_std);
+        if (plane % g.cg == 0 && threadIdx.x % THREADS == 0) {
+            mean_out[group] = mean;
+            inv_std_out[group] = inv_std;
+        }
     }
     const A scale = inv_std * gamma[c], shift = beta[c];
     T* out = y + plane * g.pixels;
@@ -1292,6 +1298,18 @@ long wave_blocks(long waves) { return (waves + kWaves - 1) / kWaves; }
 
 long plane_blocks(long planes, int threads) { return (planes + kT / threads - 1) / (kT / threads); }
 
+// The same choice as kJoinForward for channels first, where every plane would join the moments of its group's planes, by the
+// plane's threads, a wave at most.  One group in bfloat16: 64 x 2048 x 7 x 7 (512 moments a lane) 236 us and 24 joined once,
+// 64 x 1024 x 14 x 14 (64) 74 and 25, 64 x 512 x 27 x 27 (32) 43 and 37; in groups of 73, 64 x 1022 x 7 x 7 (19) 14.0 and 12.1;
+// in groups of 128, 64 x 512 x 27 x 27 (8) 36.4 and 37.0; in one group in float32, 64 x 256 x 56 x 56 (4) 101 and 104.
+constexpr long kJoinPlanes = 8;
+
+bool joined_planes(int cg, int threads)
+{
+    const int lanes = threads < kWave ? threads : kWave;
+    return (cg + lanes - 1) / lanes > kJoinPlanes;
+}
+
 unsigned eights(long blocks) { return (unsigned)((blocks + 7) / 8 * 8); }
 
 template <typename T, int ACT>
@@ -1347,10 +1365,14 @@ int forward(int nhwc, const T* x, const wide_t<T>* gamma, const wide_t<T>* beta,
     return with_plane<T>(pixels, [&](auto threads) {
         constexpr int V = 16 / sizeof(T), N = decltype(threads)::value;
         const long blocks = plane_blocks(g.planes, N);
-        if (too_many(blocks)) return PYDTNN_HIP_ERR_UNSUPPORTED;
+        const bool joined = joined_planes(cg, N);
+        if (too_many(blocks) || (joined && too_many(wave_blocks(images * groups)))) return PYDTNN_HIP_ERR_UNSUPPORTED;
         hipLaunchKernelGGL((gn_first_moments<T, V, N>), dim3((unsigned)blocks), dim3(kT), 0, st, x, part, g);
-        hipLaunchKernelGGL((gn_first_apply<T, V, N, ACT>), dim3((unsigned)blocks), dim3(kT), 0, st, x, gamma, beta, part, y,
-                           mean, inv_std, eps, g);
+        if (joined)
+            hipLaunchKernelGGL((gn_join_groups<A>), dim3((unsigned)wave_blocks(images * groups)), dim3(kT), 0, st, part, mean,
+                               inv_std, images * groups, cg, (long)cg * pixels, (long)pixels, 1, eps);
+        hipLaunchKernelGGL((gn_first_apply<T, V, N, ACT>), dim3((unsigned)blocks), dim3(kT), 0, st, x, gamma, beta,
+                           joined ? nullptr : part, y, mean, inv_std, eps, g);
         HIP_RETURN_IF_LAUNCH_FAILED();
         return PYDTNN_HIP_OK;
     });

@@ -759,3 +759,25 @@ def test_group_norm_of_one_large_image_costs_a_few_copies(ops, groups):
     backward = least_us(lambda: ops.gn_backward(dy, x, gamma, beta, mean, inv_std, groups))
     print(f"copy {copy:.1f} us, forward {forward:.1f}, backward {backward:.1f}")
     assert forward < 8 * copy and backward < 8 * copy, (copy, forward, backward)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [(3, (7, 7), 2049, 1), (2, (14, 14), 1026, 1), (2, (3, 3), 18000, 2), (1, (33, 31), 600, 1)], ids=str)
+def test_group_norm_of_groups_of_many_planes(ops, shape, dtype):
+    """Groups of more planes than a workgroup holds, whose moments a kernel of its own joins."""
+    announce("group norm, many planes", shape, dtype)
+    x, dy, gamma, beta, groups = gn_inputs(shape, dtype, False, 8)
+    check_gn(ops, x, dy, gamma, beta, groups, "silu", False)
+    check_gn(ops, misaligned(x), dy, gamma, beta, groups, "relu", False)
+
+
+def test_group_norm_of_many_small_planes_costs_a_few_copies(ops):
+    """What the planes of a group join does not grow with the square of their number: 131072 planes of 7 x 7 in one group an
+    image, 25.7 MB, take at most fifteen times what a copy takes (forward moves them three times, and each of its three launches
+    takes as long as a copy of this size)."""
+    announce("group norm, small planes")
+    x, _, gamma, beta, _ = gn_inputs((64, (7, 7), 2048, 1), torch.float32, False, 9)
+    copy = least_us(x.clone)
+    forward = least_us(lambda: ops.gn_forward(x, gamma, beta, 1, nhwc=False))
+    print(f"copy {copy:.1f} us, forward {forward:.1f}")
+    assert forward < 15 * copy, (copy, forward)
