@@ -1103,11 +1103,13 @@ GnLast last_shape(long images, int channels, int pixels, int groups, int v)
 
 // Each workgroup of a second pass joins what the runs of its slab's groups left, which grows with the square of the runs: where
 // a lane would take more than kJoinForward moments, or kJoinBackward channel sums, a kernel (backward two) of a wave a
-// group joins them once.  In float32, groups of 8, 4 x 112 x 112 x 256 (191 runs): forward 24 a lane 31 us, joined once 27;
-// backward 191 a lane 54 and 47.  8 x 112 x 112 x 256 (96 runs): forward 12 a lane 48.8 and 48.5, backward 96 a lane 82.2 and
-// 81.9; 16 x 112 x 112 x 256 (48): forward 6 a lane 92.7 and 93.1, backward 48 a lane 174.6 and 176.3.  1 x 112 x 112 x 1024 (738
-// runs): forward in groups of one 2600 and 40, backward in groups of 16 600 and 58.
-constexpr long kJoinForward = 16, kJoinBackward = 64;
+// group joins them once.  1 x 112 x 112 x 1024 in float32 (738 runs): forward in groups of one 2600 us and 41 joined once, backward in
+// groups of 16 600 and 58.  About the limits, forward in groups of 8: 4 x 112 x 112 x 256 (24 a lane) 31 and 27, 8 x 112 x 112 x 256
+// (12) 48.8 and 48.5, 16 x 112 x 112 x 256 (6) 92.7 and 93.1.  Backward: 4 x 112 x 112 x 256 in groups of 8 (191 a lane) 54 and 47;
+// 32 x 28 x 28 x 1024 in bfloat16 in groups of 16 (192) 82 and 70; 24 x 20 x 20 x 1024 in groups of 128 (128) 53 and 50, in
+// bfloat16 45 and 44; 48 x 20 x 20 x 512 in one group (128) 46 and 47, in bfloat16 39 and 42; 64 x 20 x 20 x 2048 in bfloat16 in
+// groups of 256 (96) 116 and 132.
+constexpr long kJoinForward = 16, kJoinBackward = 128;
 
 // What a lane of a workgroup joins where each group has that many entries.
 long entries_of_lane(const GnLast& g, long entries)
@@ -1299,10 +1301,11 @@ long wave_blocks(long waves) { return (waves + kWaves - 1) / kWaves; }
 long plane_blocks(long planes, int threads) { return (planes + kT / threads - 1) / (kT / threads); }
 
 // The same choice as kJoinForward for channels first, where every plane would join the moments of its group's planes, by the
-// plane's threads, a wave at most.  One group in bfloat16: 64 x 2048 x 7 x 7 (512 moments a lane) 236 us and 24 joined once,
-// 64 x 1024 x 14 x 14 (64) 74 and 25, 64 x 512 x 27 x 27 (32) 43 and 37; in groups of 73, 64 x 1022 x 7 x 7 (19) 14.0 and 12.1;
-// in groups of 128, 64 x 512 x 27 x 27 (8) 36.4 and 37.0; in one group in float32, 64 x 256 x 56 x 56 (4) 101 and 104.
-constexpr long kJoinPlanes = 8;
+// plane's threads, a wave at most.  In bfloat16: 64 x 2048 x 7 x 7 in one group (512 moments a lane) 236 us and 24 joined once,
+// 64 x 1024 x 14 x 14 (64) 74 and 25; in groups of 73, 64 x 1022 x 7 x 7 (19) 14.0 and 12.1; in groups of 51, x 1020 x 3 x 3 (13) 10.7
+// and 9.7 for 64 images, 7.7 and 8.5 for eight; in groups of 37, 64 x 148 x 7 x 7 (10) 8.1 and 9.1; in groups of 131, 128 x 1048 x 13 x
+// 13 in float32 (9) 63 and 69; in one group in float32, 64 x 256 x 56 x 56 (4) 101 and 104.
+constexpr long kJoinPlanes = 12;
 
 bool joined_planes(int cg, int threads)
 {
