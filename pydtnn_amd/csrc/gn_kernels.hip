@@ -1122,27 +1122,45 @@ bool joined_forward(const GnLast& g) { return entries_of_lane(g, g.splits) > kJo
 // (a slab that is one run joins nothing twice)
 bool joined_backward(const GnLast& g) { return g.splits > 1 && entries_of_lane(g, g.cg) * g.splits > kJoinBackward; }
 
+// Whether to take a slab of so many packs that leaves threads idle, where no other way holds one.  17 groups, two passes second.
+// Forward: where there are few workgroups (float32, 64 x 7 x 7 x 544: 8.6 us and 10.9; but 18.2 and 15.3 for 256 images) or more
+// packs than the smallest way holds (1024 x 14 x 14 x 544 160 and 223, 256 images 42 and 50).  Backward: 64 x 7 x 7 x 544 14 and 20,
+// x 3 x 3 x 544 for 120 images 15.7 and 13.1; 1024 x 14 x 14 x 544 331 and 417, in float64 with 272 channels 324 and 383, 256 of those
+// 96 and 85.
+enum class Idle { kNever, kForward, kBackward };
+
+bool takes_idle(Idle idle, long packs, long pieces)
+{
+    if (idle == Idle::kForward) return packs >= kWave && (pieces <= 2048 || packs > 1024);
+    return idle == Idle::kBackward && (packs > 1024 ? pieces > 8192 : pieces <= 2048 && packs >= 256);
+}
+
 // Where one kernel can hold a slab of an image in the registers of `threads` threads, `packs` packs of 16 bytes each (of x,
 // and in the backward pass as many of dy): the smallest slab of whole groups whose rows have at least `line` bytes, or all
-// channels; at most `most` of them.
-bool whole_shape(GnLast* g, long images, int channels, int pixels, int groups, int v, int size, int line, long most,
+// channels; at most `most` of them.  A slab of few packs leaves threads idle: it grows while there are workgroups enough.  Where no
+// wider one fits (group counts with few divisors) the way is passed over, unless `idle` says that the idle slab is better than
+// two passes.
+bool whole_shape(GnLast* g, long images, int channels, int pixels, int groups, int v, int size, int line, long most, Idle idle,
                  int threads, int packs)
 {
     if (v * size != 16) return false;
     const int cg = channels / groups;
+    long slab = 0;      // packs of the slab
+    bool is_idle = false;
     for (int sg = 1; sg <= groups && (long)sg * cg <= kWholeWidth; ++sg) {
         const int width = sg * cg;
         if (groups % sg || width % v || (width * size < line && sg != groups)) continue;
         const int tx = width / v;
-        // a slab of few packs leaves threads idle: it grows while there are workgroups enough
-        if (2l * pixels * tx < threads * packs && sg != groups && images * (groups / sg) > 1024) continue;
         if (tx > threads || (pixels + threads / tx - 1) / (threads / tx) > packs) break;
         *g = GnLast{images, pixels, channels, groups, cg, sg, width, groups / sg, tx, std::min(threads / tx, pixels), 1, pixels,
                     images * (groups / sg), 1, 1, {}};
-        set_joins(g, threads, v);
-        return g->pieces <= most && (g->pieces + 8) * threads < (1l << 32);      // (a launch counts its threads in 32 bits)
+        slab = (long)pixels * tx;
+        is_idle = 2 * slab < threads * packs && sg != groups && g->pieces > 1024;
+        if (!is_idle) break;
     }
-    return false;
+    if (!slab || (is_idle && !takes_idle(idle, slab, g->pieces))) return false;
+    set_joins(g, threads, v);
+    return g->pieces <= most && (g->pieces + 8) * threads < (1l << 32);      // (a launch counts its threads in 32 bits)
 }
 
 int check(long images, long channels, long pixels, long groups)
@@ -1159,13 +1177,13 @@ int size_of(int dtype) { return dtype == kDtypeF64 ? 8 : dtype == kDtypeF32 ? 4 
 template <int THREADS, int PACKS>
 struct Hold {};
 
-// Calls launch(line, most, threads, packs) for these ways in turn, with whole lines of `first` bytes, then with half lines of
-// 64 (forward 64 x 14 x 14 x 1024 in float32: 19 us with lines of 128, 22 with half lines), until one fits.
+// Calls launch(line, most, idle, threads, packs) for these ways in turn, with whole lines of `first` bytes, then with half lines
+// of 64 (forward 64 x 14 x 14 x 1024 in float32: 19 us with lines of 128, 22 with half lines), until one fits.
 template <typename F, int... THREADS, int... PACKS>
-bool hold_lines(int first, long most, F launch, Hold<THREADS, PACKS>...)
+bool hold_lines(int first, long most, Idle idle, F launch, Hold<THREADS, PACKS>...)
 {
     for (int line = first; line >= std::min(first, 64); line /= 2)
-        if ((launch(line, most, std::integral_constant<int, THREADS>(), std::integral_constant<int, PACKS>()) || ...))
+        if ((launch(line, most, idle, std::integral_constant<int, THREADS>(), std::integral_constant<int, PACKS>()) || ...))
             return true;
     return false;
 }
@@ -1187,16 +1205,21 @@ int first_line(long rows_bytes)
 // 156 against 187; 92 against 95).  A workgroup that has a compute unit to itself is taken where one round of them does it all:
 // forward 56 x 56 x 256 in float32 takes 22 us against 30 in two passes for 16 images (256 slabs), 103 against 102 for 64.
 // SHORT: packs of eight 16-bit values, whose sums leave registers for fewer of them (backward 64 x 28 x 28 x 512 in bfloat16:
-// 61 us in two passes, 81 with twelve packs to 512 threads).
+// 61 us in two passes, 81 with twelve packs to 512 threads); idle slabs of them lose (1024 x 10 x 10 x 544: 72 us forward, 52 in
+// two passes).
 constexpr long kAny = 1l << 40, kOneRound = 256;
 
 template <bool SHORT, typename F>
 bool hold_forward(long rows_bytes, F launch)
 {
     const int line = first_line(rows_bytes);
-    if (hold_lines(line, kAny, launch, Hold<256, 4>(), Hold<512, 8>())) return true;
-    if constexpr (SHORT) return hold_lines(128, kOneRound, launch, Hold<512, 24>());
-    else return hold_lines(line, kAny, launch, Hold<512, 16>()) || hold_lines(128, kOneRound, launch, Hold<1024, 16>());
+    if (hold_lines(line, kAny, Idle::kNever, launch, Hold<256, 4>(), Hold<512, 8>())) return true;
+    if constexpr (SHORT)
+        return hold_lines(128, kOneRound, Idle::kNever, launch, Hold<512, 24>());
+    else
+        return hold_lines(line, kAny, Idle::kNever, launch, Hold<512, 16>()) ||
+               hold_lines(128, kOneRound, Idle::kNever, launch, Hold<1024, 16>()) ||
+               hold_lines(line, kAny, Idle::kForward, launch, Hold<256, 4>(), Hold<512, 8>(), Hold<512, 16>());
 }
 
 template <bool SHORT, typename F>
@@ -1204,11 +1227,12 @@ bool hold_backward(long rows_bytes, F launch)
 {
     const int line = first_line(rows_bytes);
     if constexpr (SHORT)
-        return hold_lines(line, kAny, launch, Hold<256, 4>(), Hold<256, 8>()) ||
-               hold_lines(128, kOneRound, launch, Hold<512, 12>());
+        return hold_lines(line, kAny, Idle::kNever, launch, Hold<256, 4>(), Hold<256, 8>()) ||
+               hold_lines(128, kOneRound, Idle::kNever, launch, Hold<512, 12>());
     else
-        return hold_lines(line, kAny, launch, Hold<256, 4>(), Hold<512, 8>()) ||
-               hold_lines(line, kAny, launch, Hold<1024, 8>());
+        return hold_lines(line, kAny, Idle::kNever, launch, Hold<256, 4>(), Hold<512, 8>()) ||
+               hold_lines(line, kAny, Idle::kNever, launch, Hold<1024, 8>()) ||
+               hold_lines(line, kAny, Idle::kBackward, launch, Hold<256, 4>(), Hold<512, 8>(), Hold<1024, 8>());
 }
 
 // Calls launch(threads, packs) for the smallest workgroup whose registers hold `packs` packs of a group that is one run of
@@ -1241,9 +1265,9 @@ size_t workspace_bytes_of(int dtype, bool nhwc, bool backward, long images, int 
     const int v = aligned ? pack_of(size, channels, channels / groups) : 1;
     long moments = images * channels, sums = images * channels, joined = 0;      // pieces of groups, of channels, channels of images
     if (nhwc) {
-        auto fits = [&](int line, long most, auto threads, auto packs) {
+        auto fits = [&](int line, long most, Idle idle, auto threads, auto packs) {
             GnLast g;
-            return whole_shape(&g, images, channels, pixels, groups, v, size, line, most, threads, packs);
+            return whole_shape(&g, images, channels, pixels, groups, v, size, line, most, idle, threads, packs);
         };
         const long rows_bytes = images * channels * size;
         if (!backward && (size == 2 ? hold_forward<true>(rows_bytes, fits) : hold_forward<false>(rows_bytes, fits))) return 0;
@@ -1324,9 +1348,9 @@ int forward(int nhwc, const T* x, const wide_t<T>* gamma, const wide_t<T>* beta,
     if (nhwc) {
         const int v = aligned16(x) && aligned16(y) ? pack_of(sizeof(T), channels, channels / groups) : 1;
         GnLast g;
-        auto whole = [&](int line, long most, auto threads, auto packs) {
+        auto whole = [&](int line, long most, Idle idle, auto threads, auto packs) {
             constexpr int N = decltype(threads)::value, M = decltype(packs)::value;
-            if (!whole_shape(&g, images, channels, pixels, groups, v, sizeof(T), line, most, N, M)) return false;
+            if (!whole_shape(&g, images, channels, pixels, groups, v, sizeof(T), line, most, idle, N, M)) return false;
             hipLaunchKernelGGL((gn_last_whole<T, 16 / (int)sizeof(T), ACT, N, M>), dim3(eights(g.pieces)), dim3(N), 0, st, x,
                                gamma, beta, y, mean, inv_std, eps, g);
             return true;
@@ -1397,9 +1421,9 @@ int backward(int nhwc, const T* dy, const T* x, const wide_t<T>* gamma, const wi
     if (nhwc) {
         const int v = aligned16(x) && aligned16(dy) && aligned16(dx) ? pack_of(sizeof(T), channels, cg) : 1;
         GnLast g;
-        auto whole = [&](int line, long most, auto threads, auto packs) {
+        auto whole = [&](int line, long most, Idle idle, auto threads, auto packs) {
             constexpr int N = decltype(threads)::value, M = decltype(packs)::value;
-            if (!whole_shape(&g, images, channels, pixels, groups, v, sizeof(T), line, most, N, M)) return false;
+            if (!whole_shape(&g, images, channels, pixels, groups, v, sizeof(T), line, most, idle, N, M)) return false;
             hipLaunchKernelGGL((gn_last_bwd_whole<T, 16 / (int)sizeof(T), ACT, N, M>), dim3(eights(g.pieces)), dim3(N), 0, st,
                                dy, x, gamma, beta, mean, inv_std, sums, dx, g);
             params(images);

@@ -781,3 +781,56 @@ def test_group_norm_of_many_small_planes_costs_a_few_copies(ops):
     forward = least_us(lambda: ops.gn_forward(x, gamma, beta, 1, nhwc=False))
     print(f"copy {copy:.1f} us, forward {forward:.1f}")
     assert forward < 15 * copy, (copy, forward)
+
+
+# --------------------------------------------------------------------------- group norm: tensors too large for the host form
+def of_group(t, nhwc, images, channels):
+    return t[images][..., channels] if nhwc else t[images][:, channels]
+
+
+def check_gn_of_groups(ops, x, dy, gamma, beta, groups, activation, nhwc, samples, eps=1e-5):
+    """check_gn for a few (image, group): y, the statistics and dx of each against the 64-bit form of that group by itself,
+    dgamma and dbeta of its channels against sums in 64 bits over all images."""
+    dtype, cg = x.dtype, gamma.numel() // groups
+    y, mean, inv_std = ops.gn_forward(x, gamma, beta, groups, eps, activation, nhwc)
+    dgamma, dbeta, dx = ops.gn_backward(dy, x, gamma, beta, mean, inv_std, groups, activation, nhwc)
+    for image, group in samples:
+        at, ch = slice(image, image + 1), slice(group * cg, (group + 1) * cg)
+        hx, hdy, hg, hb = (oo.host64(t) for t in (of_group(x, nhwc, at, ch), of_group(dy, nhwc, at, ch), gamma[ch], beta[ch]))
+        ref = oo.gn_forward(hx, hg, hb, 1, eps, activation, nhwc)
+        bounds = oo.gn_forward_bounds(hx, hg, hb, 1, eps, nhwc, ref[0], dtype)
+        got = (of_group(y, nhwc, at, ch), mean[at, group:group + 1], inv_std[at, group:group + 1])
+        for g, r, b, what in zip(got, ref, bounds, ("y", "mean", "inv_std")):
+            within(g, r, b, (what, image, group))
+        hm, hi = oo.host64(got[1]), oo.host64(got[2])
+        ref = oo.gn_backward(hdy, hx, hg, hb, hm, hi, 1, activation, nhwc)[2]
+        bound = oo.gn_backward_bounds(hdy, hx, hg, hb, hm, hi, 1, activation, nhwc, ref, dtype)[2]
+        within(of_group(dx, nhwc, at, ch), ref, bound, ("dx", image, group))
+    for group in sorted({g for _, g in samples}):
+        ch = slice(group * cg, (group + 1) * cg)
+        sums = torch.zeros(4, cg, dtype=torch.float64, device=x.device)      # dz xn, dz and the magnitudes of each
+        for i in range(x.shape[0]):
+            xi, di = (of_group(t, nhwc, slice(i, i + 1), ch).double() for t in (x, dy))
+            if not nhwc:
+                xi, di = xi.transpose(1, -1), di.transpose(1, -1)
+            xi, di = xi.reshape(-1, cg), di.reshape(-1, cg)
+            xn = (xi - mean[i, group].double()) * inv_std[i, group].double()
+            z = xn * gamma[ch].double() + beta[ch].double()
+            dz = di * (z > 0) if activation == "relu" else di
+            sums += torch.stack([(dz * xn).sum(0), dz.sum(0), (dz * xn).abs().sum(0), dz.abs().sum(0)])
+        # as in gn_backward_bounds
+        u, n = oo.WIDE_HALF_STEP[dtype], x.numel() // gamma.numel()
+        k = (8 * n ** 0.5 + 8) * u
+        ref = oo.host64(sums)
+        within(dgamma[ch], ref[0], (k + 7 * u) * ref[2], ("dgamma", group))
+        within(dbeta[ch], ref[1], k * ref[3], ("dbeta", group))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64], ids=str)
+@pytest.mark.parametrize("images,pixels", [(64, (7, 7)), (500, (14, 14))])
+def test_group_norm_of_a_slab_that_leaves_threads_idle(ops, images, pixels, dtype):
+    """17 groups: one kernel holds a slab of a group, and no wider one fits."""
+    announce("group norm, idle slab", images, pixels, dtype)
+    c = 544 if dtype == torch.float32 else 272
+    x, dy, gamma, beta, groups = gn_inputs((images, pixels, c, 17), dtype, True, 3)
+    check_gn_of_groups(ops, x, dy, gamma, beta, groups, "relu", True, [(0, 0), (images // 2, 7), (images - 1, 16)])

@@ -271,3 +271,11 @@ def test_a_dropout_layers_seed_may_be_any_whole_number(seed):
     for bad in (1.5, "5", np.float32(5)):
         with pytest.raises(TypeError):
             pd.Dropout(rate=0.5, seed=bad)
+
+
+def test_gn_holds_a_slab_that_fits_where_no_wider_one_does(lib):
+    """17 and 19 groups have no divisor to make wider slabs of: forward in one kernel, which needs no workspace."""
+    for images, channels, pixels, groups in ((64, 544, 49, 17), (64, 608, 16, 19), (1024, 544, 196, 17)):
+        assert lib.pydtnn_hip_gn_workspace_bytes(0, 1, 0, images, channels, pixels, groups, 1) == 0
+    # many workgroups of a few idle packs are slower than two passes
+    assert lib.pydtnn_hip_gn_workspace_bytes(0, 1, 0, 1024, 544, 49, 17, 1) > 0
