@@ -834,3 +834,66 @@ def test_group_norm_of_a_slab_that_leaves_threads_idle(ops, images, pixels, dtyp
     c = 544 if dtype == torch.float32 else 272
     x, dy, gamma, beta, groups = gn_inputs((images, pixels, c, 17), dtype, True, 3)
     check_gn_of_groups(ops, x, dy, gamma, beta, groups, "relu", True, [(0, 0), (images // 2, 7), (images - 1, 16)])
+
+
+@pytest.mark.parametrize("activation", ["", "relu"])
+@pytest.mark.parametrize("nhwc", [True, False], ids=["last", "first"])
+def test_group_norm_of_more_than_2_to_31_elements_in_64_bits(ops, nhwc, activation):
+    """Groups of the first image and of the last, whose elements lie beyond 2^31, in either format; 32 channels and 2^18 pixels
+    a group."""
+    announce("group norm beyond 32 bits in 64 bits", nhwc, activation)
+    images, pixels, c, groups = 9, 1 << 18, 1024, 32
+    shape = (images, pixels, c) if nhwc else (images, c, pixels)
+    x, dy = (torch.empty(shape, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    for i in range(images):
+        g = torch.Generator(device="cuda").manual_seed(i)
+        x[i].normal_(mean=0.5, std=1.5, generator=g)
+        dy[i].normal_(generator=g)
+    gamma, beta = torch.rand(c, device="cuda") + 0.5, torch.randn(c, device="cuda")
+    check_gn_of_groups(ops, x, dy, gamma, beta, groups, activation, nhwc, [(0, 0), (8, 31)])
+
+
+# --------------------------------------------------------------------------- the larger tiles of the e4m3 product
+# (m, n, k) that take tiles of 256 (16-bit types; at least 192 of them) and of 128, several in each direction, ragged in every
+# extent, the last bands of tiles partly empty
+FP8_TILES = [(3000, 4099, 300), (2900, 4200, 1100), (4100, 2900, 129), (1500, 2100, 700), (2060, 1540, 1), (1800, 1795, 2050)]
+
+
+@pytest.mark.parametrize("dtype", FP8_DTYPES, ids=str)
+@pytest.mark.parametrize("shape", FP8_TILES, ids=str)
+def test_matmul_fp8_in_the_larger_tiles(ops, shape, dtype):
+    m, n, k = shape
+    announce("matmul_fp8, larger tiles", shape, dtype)
+    x, w = fp8_matrix(m, k, dtype, m + k), fp8_matrix(n, k, torch.float32, n + k) * 2.0 ** -7
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(n)).cuda()
+    wq, ws = ops.quantize_fp8(w)
+    hq, he = oo.quantize_fp8(oo.host64(w))
+    y = ops.matmul_fp8(x, wq, ws, bias=bias, relu=True)
+    plain = ops.matmul_fp8(misaligned(x), wq, ws)
+    # rows of every tile and the ragged ends, all columns
+    rows = sorted({*range(0, m, 37), *range(0, m, 64), *range(63, m, 64), *range(max(0, m - 20), m)})
+    hx, hy = oo.host64(x[rows]), oo.host64(y[rows])
+    ref, bound = oo.matmul_fp8(hx, hq, he, oo.host64(bias), True, dtype)
+    within(y[rows], ref, bound, "y")
+    assert np.linalg.norm(hy - ref) <= (oo.HALF_STEP[dtype] + 2.0 ** -13) * np.linalg.norm(ref)
+    ref, bound = oo.matmul_fp8(hx, hq, he, None, False, dtype)
+    within(plain[rows], ref, bound, "y without bias")
+    # every other row: as the same rows in another order, which puts them in other places of other tiles
+    order = torch.randperm(m, generator=torch.Generator().manual_seed(k)).cuda()
+    assert torch.equal(ops.matmul_fp8(x[order], wq, ws, bias=bias, relu=True), y[order])
+
+
+@pytest.mark.parametrize("shape", [(131100, 16, 16400), (50001, 43003, 128), (3, 131100, 16400), (40, 131100, 16400)], ids=str)
+def test_matmul_fp8_of_more_than_2_to_31_elements(ops, shape):
+    """Activations, results and weights (for a few rows and for more) beyond 2^31 elements: their first and last rows."""
+    m, n, k = shape
+    announce("matmul_fp8 beyond 32 bits", shape)
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x = torch.empty((m, k), dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    w = torch.empty((n, k), dtype=torch.bfloat16, device="cuda").normal_(std=2.0 ** -7, generator=g)
+    y = ops.matmul_fp8(x, *ops.quantize_fp8(w))
+    rows = sorted({0, 1, m // 2, *range(max(0, m - 12), m)} & set(range(m)))
+    columns = sorted({0, 1, n // 2, *range(max(0, n - 20), n)} & set(range(n)))
+    hq, he = oo.quantize_fp8(oo.host64(w[columns]))
+    ref, bound = oo.matmul_fp8(oo.host64(x[rows]), hq, he, None, False, torch.bfloat16)
+    within(y[rows][:, columns], ref, bound, "y")
