@@ -446,6 +446,7 @@ int pydtnn_hip_bn_training_bwd_f64(const double *dy, const double *xn, const dou
  * (images, channels, pixels); a group is channels / groups consecutive channels over all pixels of an image.
  *   forward : mean, inv_std = 1 / sqrt(var + eps) of each group (images, groups), var without Bessel's correction;
  *             z = gamma[c] * (x - mean) * inv_std + beta[c];  y = z, z > 0 ? z : 0 or z / (1 + exp(-z)).
+ *             In float32 and 16-bit types 1 / (1 + exp(-z)) is within (3 + |z|) 2^-23 of itself, and 0 for z under -87.34.
  *   backward: from dy, x and the forward's mean and inv_std: dgamma, dbeta (channels) and, unless it is NULL, dx.
  *             Where the activation is PYDTNN_HIP_ACT_RELU, dy counts where z, computed from these inputs, is positive.
  * Sums are taken in a fixed order.  Outputs may not overlap inputs.  channels has to be a multiple of groups; pixels and

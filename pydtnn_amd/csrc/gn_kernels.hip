@@ -33,7 +33,8 @@ constexpr int kWholeWidth = 512;      // channels of a slab that one kernel hold
 enum { kIdentity = 0, kRelu = 1, kSilu = 2 };
 
 // 1 / (1 + e^-z).  In 32 bits through the hardware's 2^v and 1/v, each within a step: their errors and that of the product
-// -z log2(e) move the result by a few steps of 1 + |z|.
+// -z log2(e) move the result by at most 3 + |z| steps.  Under z = -126 log 2 = -87.34 the reciprocal is below the smallest normal
+// number and counts as 0.
 __device__ __forceinline__ float sigmoid(float z)
 {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f));

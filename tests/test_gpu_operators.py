@@ -897,3 +897,28 @@ def test_matmul_fp8_of_more_than_2_to_31_elements(ops, shape):
     hq, he = oo.quantize_fp8(oo.host64(w[columns]))
     ref, bound = oo.matmul_fp8(oo.host64(x[rows]), hq, he, None, False, torch.bfloat16)
     within(y[rows][:, columns], ref, bound, "y")
+
+
+def test_group_norm_silu_is_as_exact_as_its_documentation_says(ops):
+    """Constant groups, whose z is the shift itself: 1 / (1 + exp(-z)) within (3 + |z|) steps of 2^-23 (the hardware's 2^v and
+    1/v a step each, the sum half a step, the exponent's rounding 0.63 |z| of a step), one more half step for the product, and 0
+    under -126 log 2, where 1 + exp(-z) is over 2^126 and its reciprocal below the smallest normal number; its derivative
+    p (1 + z (1 - p)) with p off by as much and three roundings of (1 + |z|)."""
+    announce("group norm silu")
+    z = np.concatenate([np.linspace(-87.3, 88.7, 6001), np.linspace(-3, 3, 2001), [-1e4, -200.0, -104.0, -88.0, -87.5, 200.0, 1e4],
+                        [0.0, 2.0 ** -60, -2.0 ** -60, 2.0 ** -140]])
+    beta = torch.from_numpy(z).float().cuda()
+    z = oo.host64(beta)
+    c = len(z)
+    x, gamma = torch.full((1, 1, c), 2.5, device="cuda"), torch.ones(c, device="cuda")
+    y, mean, inv_std = ops.gn_forward(x, gamma, beta, c, 1e-5, "silu")
+    with np.errstate(over="ignore"):
+        p = 1 / (1 + np.exp(-z))
+    e = (3 + np.abs(z)) * 2.0 ** -23
+    low = z < -126 * np.log(2)      # -87.3365
+    got = oo.host64(y).reshape(-1)
+    assert np.all(got[low] == 0)
+    assert np.all(np.abs(got - z * p)[~low] <= ((e + 2.0 ** -24) * np.abs(z * p) + 2.0 ** -149)[~low])
+    dbeta = oo.host64(ops.gn_backward(torch.ones_like(x), x, gamma, beta, mean, inv_std, c, "silu")[1])
+    bound = p * (e * np.abs(1 + z * (1 - p)) + np.abs(z) * p * e + (1 + np.abs(z)) * 2.0 ** -22) + 2.0 ** -149
+    assert np.all(np.abs(dbeta - p * (1 + z * (1 - p)))[~low] <= bound[~low]) and np.all(dbeta[low] == 0)
