@@ -473,7 +473,8 @@ int pydtnn_hip_gn_backward(int dtype, int nhwc, const void *dy, const void *x, c
  * (to even between two), an element is kept when its number is >= threshold and then multiplied by
  * 2^16 / (2^16 - threshold), the reciprocal of the probability that it is kept; it is 0 otherwise, whatever x holds.
  * `offset_dev`, unless it is NULL, is a number on the device that is added to `offset`: a captured graph whose number
- * changes between replays draws another mask each time.  y may be x.  0 <= rate <= 1. */
+ * changes between replays draws another mask each time.  y may be x.  0 <= rate <= 1.  total is at most 2^35 - 2^11
+ * (PYDTNN_HIP_ERR_UNSUPPORTED: a launch has fewer than 2^32 threads). */
 int pydtnn_hip_dropout(int dtype, const void *x, void *y, long total, double rate, uint64_t seed, uint64_t offset,
                        const int64_t *offset_dev, void *stream);
 

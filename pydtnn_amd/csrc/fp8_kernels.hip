@@ -9,13 +9,18 @@
 //   16-bit results: v_mfma_scale_f32_16x16x128_f8f6f4, twice the rate of the 16-bit instructions.  It adds its products in
 //       eights, each aligned to the largest of the eight with 13 bits below that one's leading bit (measured with powers of
 //       two; eights are then added in 32 bits): a relative error of 1e-5 of a sum of like signs, a fortieth of the half
-//       step that a float16 result is rounded by.
+//       step that a float16 result is rounded by.  4096 x 4096 x 4096 in bfloat16 lies 2.0e-4 of its norm from sums of 24 bits
+//       rounded alike, and 1.66e-3 from the result in 64 bits, as those do: that is its own rounding.
 //   float32 results: the operands are converted to bfloat16 with their scales, which is exact, and go through
-//       v_mfma_f32_16x16x32_bf16, which keeps 24 bits of everything it adds.
+//       v_mfma_f32_16x16x32_bf16, which keeps 24 bits of everything it adds (4096 x 4096 x 4096: 126 us, 68 in bfloat16).
 //
 // Layout: q is (rows, k to a multiple of 128), zeros behind k; scales is (rows, blocks to a multiple of 4), one byte e + 127
 // each, 127 behind the last block, so that a lane fetches the scales of four blocks as one word.
 // A block that holds an infinity or a NaN is NaN throughout, with scale 1.
+//
+// Times below, unless they are the product's alone, are of whole calls in a replayed graph, inputs from three sets in turn.  Rows of
+// a thousand calls without a graph take less where a call is long (4096 x 4096 x 4096 in bfloat16 68 us, 72 in the graph; 16 x 25088 x
+// 4096 32 and 35) and more where it is short, by what a call costs the host (1 x 4096 x 1000 10 and 6).
 #include "../../include/pydtnn_hip.h"
 #include "conv_internal.h"
 #include "dtypes.h"
@@ -179,7 +184,7 @@ __device__ __forceinline__ RowsWords rows_words(const void* base, long bytes)
 //
 // Where local memory holds all of x (kFewLocal bytes), every workgroup quantises it for itself, while its first weights
 // are on their way: one launch instead of two (1 x 4096 x 1000 in float32: 5.8 us, 7.4 with two).  Otherwise x comes quantised.
-// 16 x 4096 x 1000 in float32 takes 9 us, 12 in tiles; 8 x 4096 x 4096 9.5 and 13; 16 x 25088 x 4096 34 and 38, where the
+// 16 x 4096 x 1000 in float32 takes 9 us, 12 in tiles; 8 x 4096 x 4096 9.5 and 13; 16 x 25088 x 4096 35 and 38, where the
 // weights arrive at 3.6 TB/s beside as many bytes of x from the second-level cache.
 constexpr int kFewWaves = 8, kFewLocal = 32 * 1024;
 

@@ -279,3 +279,8 @@ def test_gn_holds_a_slab_that_fits_where_no_wider_one_does(lib):
         assert lib.pydtnn_hip_gn_workspace_bytes(0, 1, 0, images, channels, pixels, groups, 1) == 0
     # many workgroups of a few idle packs are slower than two passes
     assert lib.pydtnn_hip_gn_workspace_bytes(0, 1, 0, 1024, 544, 49, 17, 1) > 0
+
+
+def test_dropout_refuses_a_launch_of_too_many_threads(lib):
+    p = ctypes.c_void_p(FAKE)
+    assert lib.pydtnn_hip_dropout(3, p, p, (1 << 35) - (1 << 11) + 1, 0.5, 1, 0, None, None) == 4
