@@ -922,3 +922,38 @@ def test_group_norm_silu_is_as_exact_as_its_documentation_says(ops):
     dbeta = oo.host64(ops.gn_backward(torch.ones_like(x), x, gamma, beta, mean, inv_std, c, "silu")[1])
     bound = p * (e * np.abs(1 + z * (1 - p)) + np.abs(z) * p * e + (1 + np.abs(z)) * 2.0 ** -22) + 2.0 ** -149
     assert np.all(np.abs(dbeta - p * (1 + z * (1 - p)))[~low] <= bound[~low]) and np.all(dbeta[low] == 0)
+
+
+def test_group_norm_whose_sums_are_joined_once_in_graphs_and_on_two_streams(ops):
+    """The forms with kernels between their two passes, captured, replayed and called at once."""
+    announce("group norm joined, graphs and streams")
+    cases = [(gn_inputs((1, (90, 88), 520, 520), torch.float32, True, 31), True),
+             (gn_inputs((3, (7, 7), 2049, 1), torch.float32, False, 32), False)]
+
+    def both(case, nhwc):
+        x, dy, gamma, beta, groups = case
+        y, mean, inv_std = ops.gn_forward(x, gamma, beta, groups, activation="relu", nhwc=nhwc)
+        return (y, mean, inv_std, *ops.gn_backward(dy, x, gamma, beta, mean, inv_std, groups, "relu", nhwc))
+
+    eager = [both(*case) for case in cases]
+    torch.cuda.synchronize()
+    graphs = []
+    for case in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = both(*case)
+        graphs.append((graph, out))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(4):
+        for _, out in graphs:
+            for t in out:
+                t.zero_()
+        torch.cuda.synchronize()
+        again = []
+        for stream, (graph, _), case in zip(streams, graphs, cases):
+            with torch.cuda.stream(stream):
+                graph.replay()
+                again.append(both(*case))
+        torch.cuda.synchronize()
+        for (_, out), now, ref in zip(graphs, again, eager):
+            assert all(torch.equal(t, r) for t, r in zip(out, ref)) and all(torch.equal(t, r) for t, r in zip(now, ref))
